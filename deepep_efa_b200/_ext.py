@@ -39,12 +39,16 @@ CUDA_SOURCES = [
     "kernels/train_ops.cu",
     "kernels/sf_atoms.cu",
     "kernels/fused.cu",
+    "kernels/norm.cu",
+    "kernels/router.cu",
+    "kernels/few_tokens.cu",
 ]
 CPP_SOURCES = [
     "host/bindings.cpp",
     "host/gemm_bindings.cpp",
     "host/hier_bindings.cpp",
     "host/fused_bindings.cpp",
+    "host/block_bindings.cpp",
 ]
 
 CUDA_FLAGS = [

@@ -897,6 +897,7 @@ py::dict ll_layout(Runtime* rt, int num_max_tokens, int hidden, int num_experts)
 void bind_gemm(py::module_& m);  // gemm_bindings.cpp
 void bind_hier(py::module_& m);  // hier_bindings.cpp
 void bind_fused(py::module_& m); // fused_bindings.cpp
+void bind_block(py::module_& m); // block_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "deepep_efa_b200 native runtime (sm_100a)";
@@ -996,4 +997,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     bind_gemm(m);
     bind_hier(m);
     bind_fused(m);
+    bind_block(m);
 }

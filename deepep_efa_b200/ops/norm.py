@@ -1,0 +1,100 @@
+"""Root-mean-square norm of the residual stream in front of a block of experts (kernels in csrc/kernels/norm.cu).
+
+    total = x + residual                        rounded to the stream's bf16
+    y     = total * weight / sqrt(mean(total ** 2) + eps)
+
+``rms_norm`` has gradients; ``rms_norm_fp8`` is for serving and also gives the normed rows as ``(e4m3, fp32 scales per 128 channels)``, the form that
+``Buffer.dispatch`` and ``MoELayer.forward_fp8`` take. CPU tensors are computed by PyTorch operations, so that a layer runs under gloo.
+
+The reference library has no model code and so no counterpart.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _ext
+
+
+def _total(x: torch.Tensor, residual: Optional[torch.Tensor]) -> torch.Tensor:
+    return x if residual is None else (x.float() + residual.float()).to(x.dtype)
+
+
+def _check_cpu(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor]) -> None:
+    if weight.dim() != 1 or weight.size(0) != x.size(-1):
+        raise ValueError("deepep_efa_b200.rms_norm: weight must be [H]")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError("deepep_efa_b200.rms_norm: residual must be of x's shape and type")
+
+
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.size(-1))
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.eps, ctx.has_residual = eps, residual is not None
+        ctx.set_materialize_grads(False)
+        if x.is_cuda:
+            y, _, _, total = _ext.load().rms_norm(x, weight, residual, eps, True, False, False)
+        else:
+            _check_cpu(x, weight, residual)
+            total = None if residual is None else _total(x, residual)
+            t = (x if residual is None else total).float()
+            y = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()).to(x.dtype)
+        ctx.save_for_backward(x if residual is None else total, weight)
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    def backward(ctx, dy, dtotal=None):
+        total, weight = ctx.saved_tensors
+        if dy is None:
+            dx, dw = dtotal, None
+        elif total.is_cuda:
+            dx, dw = _ext.load().rms_norm_bwd(total, weight, dy, dtotal, ctx.eps)
+        else:
+            t, g = total.float(), dy.float()
+            r = torch.rsqrt(t.square().mean(-1, keepdim=True) + ctx.eps)
+            wg = g * weight.float()
+            dx = r * (wg - t * r * r * (wg * t).mean(-1, keepdim=True))
+            dx = (dx if dtotal is None else dx + dtotal.float()).to(total.dtype)
+            dw = (g * t * r).sum(0).to(weight.dtype)
+        return dx, dw, dx if ctx.has_residual else None, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """The norm of the rows of ``x`` (bf16 ``[..., H]``, ``H`` a multiple of 8 up to 32768; ``weight`` bf16 or fp32 ``[H]``). Returns ``y``, or with a ``residual``
+    of ``x``'s shape ``(y, x + residual)``. Differentiable in all three; ``weight``'s gradient is summed in fp32 in a fixed order and has its type."""
+    shape = x.shape
+    if x.dim() == 2:
+        return _RMSNorm.apply(x, weight, residual, eps)
+    out = _RMSNorm.apply(_rows(x), weight, _rows(residual), eps)
+    return out.view(shape) if residual is None else (out[0].view(shape), out[1].view(shape))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6, round_scale: bool = False,
+                 keep_rows: bool = True) -> Tuple[Tuple[torch.Tensor, torch.Tensor], Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """The norm for serving (no gradients): ``((q, scales), y, total)`` for bf16 ``x`` ``[N, H]``, ``H`` a multiple of 128.
+
+    ``q`` e4m3 ``[N, H]`` and ``scales`` fp32 ``[N, H / 128]`` are made from the normed values in fp32 as the dispatch casts its rows (largest magnitude of 128
+    channels, at least 1e-4, over 448; with ``round_scale`` rounded up to a power of two). ``y`` is bf16, None without ``keep_rows``; ``total`` is None without ``residual``."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        raise ValueError("deepep_efa_b200.rms_norm_fp8: forward only; call it under torch.no_grad()")
+    if x.is_cuda:
+        y, q, scales, total = _ext.load().rms_norm(x, weight, residual, eps, keep_rows, True, round_scale)
+        return (q, scales), y, total
+    _check_cpu(x, weight, residual)
+    if x.dim() != 2 or x.size(1) % 128 != 0:
+        raise ValueError("deepep_efa_b200.rms_norm_fp8: x must be [N, H] with H a multiple of 128")
+    total = _total(x, residual)
+    t = total.float()
+    v = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()
+    amax = v.view(v.size(0), -1, 128).abs().amax(-1).clamp(min=1e-4)
+    scales, inv = amax / 448.0, 448.0 / amax
+    if round_scale:
+        scales = torch.exp2(torch.ceil(torch.log2(scales)))
+        inv = 1.0 / scales
+    q = (v.view(v.size(0), -1, 128) * inv.unsqueeze(-1)).view(v.shape).to(torch.float8_e4m3fn)
+    return (q, scales), v.to(x.dtype) if keep_rows else None, None if residual is None else total
