@@ -10,6 +10,9 @@
 
 namespace py = pybind11;
 
+torch::Tensor gemm_error_flag(int device);               // gemm_bindings.cpp
+long long gemm_wait_cycles(int device, double timeout_ms);
+
 namespace {
 
 #define DXB_CHECK(cond, what, msg)                                                                      \
@@ -196,7 +199,6 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     c10::cuda::CUDAGuard guard(dev);
     const torch::Tensor x = fitting(x_in), idx = idx_in.contiguous(), weights = weights_in.contiguous();
     const torch::Tensor y = out.has_value() ? *out : torch::empty({T, H}, x.options().requires_grad(false));
-    const torch::Tensor h = torch::empty({T * idx.size(1), I}, x.options().requires_grad(false));
     dx::FewTokensArgs a{};
     a.x = x.data_ptr();
     a.x_stride = x.stride(0);
@@ -206,7 +208,6 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     a.w2 = w2.data_ptr();
     a.s13 = fp8 ? s13->data_ptr<float>() : nullptr;
     a.s2 = fp8 ? s2->data_ptr<float>() : nullptr;
-    a.h = h.data_ptr();
     a.out = y.data_ptr();
     a.first = first;
     a.tokens = (int)T;
@@ -215,7 +216,11 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     a.hidden = (int)H;
     a.inter = (int)I;
     a.fp8 = fp8;
-    launched(dx::launch_few_tokens(a, stream_of(x)), what);
+    a.error_flag = gemm_error_flag(dev.index()).data_ptr<int>();
+    a.wait_limit = gemm_wait_cycles(dev.index(), 2000.0);
+    const torch::Tensor scratch = torch::empty({(int64_t)dx::few_tokens_scratch(a)}, x.options().dtype(torch::kUInt8).requires_grad(false));
+    a.scratch = scratch.data_ptr();
+    launched(dx::launch_few_tokens(a, sms_of(x), stream_of(x)), what);
     return y;
 }
 

@@ -548,6 +548,10 @@ std::string bf16_form(int64_t rows, int64_t groups, int64_t n, int64_t k, bool m
     return cap != 0 ? "columns " + std::to_string(cap) : dx::rows_on_pairs(p) ? "row pairs" : "rows";
 }
 
+// For the other kernels with bounded waits: the device's error word, and how many cycles a wait may take.
+torch::Tensor gemm_error_flag(int device) { return error_flag(device); }
+long long gemm_wait_cycles(int device, double timeout_ms) { return (long long)(timeout_ms * (double)clock_khz(device)); }
+
 void bind_gemm(py::module_& m) {
     m.def("bf16_form", &bf16_form, py::arg("rows"), py::arg("groups"), py::arg("n"), py::arg("k"), py::arg("mn_major") = false, py::arg("ends") = false,
           py::arg("zero_tail") = false, py::arg("num_sms") = 148);

@@ -75,11 +75,15 @@ struct FewTokensArgs {
     const void* w2;           // [experts, hidden, inter]
     const float* s13;         // fp8: [experts, 2 inter / 128, hidden / 128]
     const float* s2;          // fp8: [experts, hidden / 128, inter / 128]
-    void* h;                  // scratch: bf16 [tokens * topk, inter]
+    void* scratch;            // few_tokens_scratch() bytes, 256-byte aligned, for this call alone
+    void* h;                  // (the launcher's: where the hidden values are)
     void* out;                // bf16 [tokens, hidden]
     int64_t first;
     int tokens, topk, experts, hidden, inter, fp8;
+    int* error_flag;          // set where a wait for a copy ran out
+    long long wait_limit;     // cycles
 };
-cudaError_t launch_few_tokens(const FewTokensArgs& a, cudaStream_t stream);
+size_t few_tokens_scratch(const FewTokensArgs& a);
+cudaError_t launch_few_tokens(const FewTokensArgs& a, int num_sms, cudaStream_t stream);
 
 }  // namespace dx
