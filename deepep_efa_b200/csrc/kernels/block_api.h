@@ -76,7 +76,6 @@ struct FewTokensArgs {
     const float* s13;         // fp8: [experts, 2 inter / 128, hidden / 128]
     const float* s2;          // fp8: [experts, hidden / 128, inter / 128]
     void* scratch;            // few_tokens_scratch() bytes, 256-byte aligned, for this call alone
-    void* h;                  // (the launcher's: where the hidden values are)
     void* out;                // bf16 [tokens, hidden]
     int64_t first;
     int tokens, topk, experts, hidden, inter, fp8;

@@ -3,24 +3,27 @@
 //   h[p]   = weights[p] silu(G[e] x[t]) * (U[e] x[t])      p = (t, k), e = idx[t, k]: rows of G and U against the tokens of their expert
 //   out[t] = sum_k W2[e] h[t, k]
 //
-// Bound by reading the chosen experts' weights once. A work unit is 32 rows of weights (16 of gate and the 16 of up that go with them, or 32 of W2) against the
-// selections of one expert, up to eight: the rows are the M operand of mma.sync m16n8k16, the selections its eight columns. (tcgen05 multiplies 128 rows at the
-// least and takes both operands in one type: here weights in e4m3 meet activations in bf16, and units of 128 rows leave most SMs without work where a token
+// Bound by reading the chosen experts' weights once. 32 rows of weights (16 of gate and the 16 of up that go with them, or 32 of W2) are multiplied with the
+// selections of one expert, up to eight at a time: the rows are the M operand of mma.sync m16n8k16, the selections its eight columns. (tcgen05 multiplies 128 rows at
+// the least and takes both operands in one type: here weights in e4m3 meet activations of 16 bits, and tiles of 128 rows leave most SMs without work where a token
 // meets eight experts. The tensor cores are idle most of the time either way.)
 //
-// A warp is a pipeline of its own: it takes every eighth box (128 bytes of each of the unit's rows, 4 KB, one TMA copy with 128-byte swizzle) through a ring
-// that only it fills and empties, over the borders of units. So no thread waits for a loader, and the eight partial sums of a unit meet in shared memory. The
-// activations' fragments come straight from L2 (a few rows, used by every unit). Since both operands may take the reduction's index in any order as long as they agree, lane t of a
-// row's four reads 16 bytes at a time (eight weights in bf16, sixteen in e4m3) and treats them as the fragments of two or four steps; rows are dealt to lanes so
-// that a quarter warp reads all 32 banks.
+// A warp is a pipeline of its own: it takes its share of the boxes (128 bytes of each of 32 rows, 4 KB, one TMA copy with 128-byte swizzle) through a ring that only it
+// fills and empties, over the borders of experts. So no thread waits for a loader. The activations' fragments come straight from L2 (a few rows, which every
+// CTA reads). Since both operands may take the reduction's index in any order as long as they agree, lane t of a row's four reads 16 bytes at a time (eight
+// weights in bf16, sixteen in e4m3) and treats them as the fragments of two or four steps; rows are dealt to lanes so that a quarter warp reads all 32 banks.
 //
-// e4m3 becomes bf16 in registers (exactly), and each 128 x 128 block's sum is scaled in fp32. The hidden values are kept as two bf16 numbers, a rounding and
-// its remainder, whose products go to the same accumulators: 16 bits of significand for one more mma per step.
+// First launch: 16 + 16 rows of one expert are a unit, which a team of warps shares; their partial sums meet in shared memory. Second launch: a CTA (or a cluster
+// of up to eight, where there are few result rows) has 32 result rows and goes through the experts of all tokens; every warp adds up its own sums per token, which
+// meet at the end, in a fixed order. So nothing is exchanged through memory but h, and no result depends on an order of arrival. The second launch begins
+// while the first one ends (programmatic dependent launch): it plans, fills its rings with weights, and only then waits for h.
 //
-// The second launch begins while the first one ends (programmatic dependent launch): it plans, fills its rings with weights, and only then waits for h. Its sums per selection
-// go to a scratch matrix; the CTA that finishes the last unit of 32 result rows adds them up over the selections of each token, in rising k: no result depends on
-// the order of arrival.
+// Types: e4m3 becomes bf16 (first launch) or fp16 (second) in registers, exactly, and each 128 x 128 block's sum is scaled in fp32. h has more bits than bf16, so that its rounding
+// is small beside that of the result: next to bf16 weights two bf16 numbers, a rounding and its remainder, whose products go to the same accumulators; next to
+// e4m3 weights fp16 with a power of two per 16 values.
 #include <cuda.h>
+
+#include <cuda_fp16.h>
 
 #include "block_api.h"
 #include "launch.cuh"
@@ -32,93 +35,130 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kUnitRows = 32;
-constexpr int kBoxBytes = kUnitRows * 128;
-constexpr int kStages = 3;
-constexpr int kCols = 8;  // selections of a unit
+constexpr int kBoxRows = 32;
+constexpr int kBoxBytes = kBoxRows * 128;
+constexpr int kMostStages = 3;
+constexpr int kCols = 8;  // selections that are multiplied at a time
 constexpr int kMaxPairs = kFewMaxTokens * kFewMaxTopk;
-constexpr int kRedBytes = kWarps * 2 * 32 * 16;
+constexpr int kTeamWarps = 4;  // warps that share a unit of the first launch
 
-struct Smem {
-    uint8_t ring[kWarps][kStages][kBoxBytes];  // 1024-byte aligned: the swizzle goes by address
-    union {
-        float4 red[kWarps][2][32];  // a unit's partial sums
-        int start[kFewMaxExperts];  // while planning: selections per expert, then where they start
-    };
-    uint16_t pair[kMaxPairs];       // selections t * topk + k in the order of their experts
-    uint16_t group_expert[kMaxPairs], group_start[kMaxPairs];  // a unit's columns: up to eight selections of one expert
-    uint64_t full[kWarps][kStages];
+// What a CTA plans by: the selections in the order of their experts, and groups of up to eight of one expert.
+struct Plan {
+    uint16_t pair[kMaxPairs];  // selection t * topk + k
+    uint16_t group_expert[kMaxPairs], group_start[kMaxPairs];
+    uint64_t full[kWarps][kMostStages];
     int warp_sum[kWarps];
-    int num_groups, num_pairs, last, abort;
+    int num_groups, num_pairs, repeated, abort;
 };
-static_assert(sizeof(float4[kWarps][2][32]) == kRedBytes && kRedBytes >= kFewMaxExperts * 4, "");
+// In front of it the rings (1024-byte aligned: the swizzle goes by address) and fp32 sums, which while planning hold where experts start: the first launch's partial
+// sums of a unit, or the second's per warp, token and row.
+__host__ __device__ constexpr size_t ring_bytes(int stages) { return (size_t)kWarps * stages * kBoxBytes; }
+__host__ __device__ constexpr size_t sum_bytes(bool up, int tokens) {
+    const size_t n = up ? (size_t)kWarps * 2 * 32 * 16 : (size_t)kWarps * tokens * kBoxRows * 4;
+    return n < kFewMaxExperts * 4 ? kFewMaxExperts * 4 : n;
+}
+// Two CTAs fit an SM: 3 x 32 KB of weights on their way in each, or 2 x 32 KB where the sums of more than eight tokens need the room.
+__host__ __device__ constexpr int stages_for(bool up, int tokens) { return up || tokens <= 8 ? 3 : 2; }
+__host__ __device__ constexpr size_t smem_bytes(bool up, int tokens) {
+    return ring_bytes(stages_for(up, tokens)) + sum_bytes(up, tokens) + sizeof(Plan);
+}
+static_assert(2 * (smem_bytes(true, 1) + 1024) <= 228 * 1024 && 2 * (smem_bytes(false, 8) + 1024) <= 228 * 1024 && 2 * (smem_bytes(false, kFewMaxTokens) + 1024) <= 228 * 1024,
+              "two CTAs share an SM");
 
 struct FewParams {
     FewTokensArgs a;
-    float* y;       // [tokens * topk, hidden]: W2[e] h[p]
-    int* finished;  // [ceil(hidden / 32)]: units done of each 32 result rows
-    int* error_flag;
+    void* h;         // bf16 weights: [2][tokens * topk, inter] bf16, roundings and remainders; e4m3: [tokens * topk, inter] fp16
+    float* h_scale;  // e4m3: [tokens * topk, inter / 16], powers of two
     long long limit;
+    int cluster;     // second launch: CTAs that share 32 result rows
 };
 
-__device__ __forceinline__ void tma_load_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int c0, int c1, int c2, int c3, bool up) {
-    if (up)
-        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-                     "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-                     "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c3)
-                     : "memory");
+__device__ __forceinline__ void tma_load_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int c0, int c1, int c2) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_box(const CUtensorMap* map, uint32_t bar, uint32_t dst, int c0, int c1, int c2, int c3) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+                 : "memory");
 }
 __device__ __forceinline__ int4 lds128(uint32_t at) {
     int4 v;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
     return v;
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ float ld_cluster_f32(const float* own, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(own)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
 }
-// Four e4m3 numbers as two pairs in bf16, which holds each of them: bytes 0 and 1, bytes 2 and 3.
+template <bool kHalf>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (kHalf)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 numbers as two pairs (bytes 0 and 1, bytes 2 and 3) in fp16 or bf16, which hold each of them, NaN included.
+__device__ __forceinline__ void e4m3x4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t half2_to_bf16x2(uint32_t v) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return f2_to_bf16x2(f.x, f.y);
+}
 __device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    uint32_t l, h;
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(l), "=r"(h) : "r"(w));
-    const float2 fl = __half22float2(*reinterpret_cast<__half2*>(&l)), fh = __half22float2(*reinterpret_cast<__half2*>(&h));
-    lo = f2_to_bf16x2(fl.x, fl.y);
-    hi = f2_to_bf16x2(fh.x, fh.y);
+    e4m3x4_to_half(w, lo, hi);
+    lo = half2_to_bf16x2(lo);
+    hi = half2_to_bf16x2(hi);
 }
-__device__ __forceinline__ int local_expert(const FewTokensArgs& a, int64_t id) {
-    const int64_t e = id - a.first;
-    return id >= 0 && e >= 0 && e < a.experts ? (int)e : -1;
+__device__ __forceinline__ uint32_t scale_half2(uint32_t v, __half2 by) {
+    const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), by);
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// Lists the selections by expert and cuts each expert's into groups of up to eight. Every CTA does this for itself: at most 1024 ids. The selections of an
-// expert that has one group come in any order (a column's result does not depend on its place); those of one that has more are sorted, since all CTAs have to
-// cut them alike.
-__device__ __forceinline__ void plan(const FewTokensArgs& a, Smem& s) {
+// Lists the selections by expert and cuts each expert's into groups of up to eight. Every CTA does this for itself: at most 1024 ids. Where a token names an
+// expert twice, the first of the selections stands for both (the first launch adds up their weights). The selections of an expert that has one group come in any order
+// (a column's result does not depend on its place); those of one that has more are sorted, since all CTAs have to cut them alike.
+__device__ __forceinline__ void make_plan(const FewTokensArgs& a, Plan& s, int* start) {
+    constexpr int kOwn = kMaxPairs / kThreads, kEach = kFewMaxExperts / kThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.tokens * a.topk;
-    int e[kMaxPairs / kThreads];
+    int e[kOwn], repeated = 0;
 #pragma unroll
-    for (int j = 0; j < kMaxPairs / kThreads; ++j) {
+    for (int j = 0; j < kOwn; ++j) {
         const int p = j * kThreads + tid;
-        e[j] = p < pairs ? local_expert(a, a.idx[p]) : -1;
+        e[j] = -1;
+        if (p >= pairs) continue;
+        const int64_t id = a.idx[p], local = id - a.first;
+        if (id < 0 || local < 0 || local >= a.experts) continue;
+        e[j] = (int)local;
+        int before = 0;
+        for (int k = p % a.topk; k > 0; --k) before |= a.idx[p - k] == id;
+        if (before) {
+            e[j] = -1;
+            repeated = 1;
+        }
     }
-    for (int i = tid; i < a.experts; i += kThreads) s.start[i] = 0;
-    __syncthreads();
+    for (int i = tid; i < a.experts; i += kThreads) start[i] = 0;
+    repeated = __syncthreads_or(repeated);
 #pragma unroll
-    for (int j = 0; j < kMaxPairs / kThreads; ++j)
-        if (e[j] >= 0) atomicAdd(&s.start[e[j]], 1);
+    for (int j = 0; j < kOwn; ++j)
+        if (e[j] >= 0) atomicAdd(start + e[j], 1);
     __syncthreads();
     // four experts per thread: exclusive sums of selections (low half) and groups (high half)
-    constexpr int kEach = kFewMaxExperts / kThreads;
     int n[kEach], sum = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         const int i = tid * kEach + j;
-        n[j] = i < a.experts ? s.start[i] : 0;
-        sum += n[j] + ((n[j] + kCols - 1) / kCols << 16);
+        n[j] = i < a.experts ? start[i] : 0;
+        sum += n[j] + (((n[j] + kCols - 1) / kCols) << 16);
     }
     const int incl = warp_incl_scan(sum);
     if (lane == 31) s.warp_sum[warp] = incl;
@@ -132,295 +172,488 @@ __device__ __forceinline__ void plan(const FewTokensArgs& a, Smem& s) {
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         const int i = tid * kEach + j;
-        if (i < a.experts) s.start[i] = before & 0xffff;
+        if (i < a.experts) start[i] = before & 0xffff;
         int g = before >> 16;
         for (int c = 0; c < n[j]; c += kCols, ++g) {
             s.group_expert[g] = (uint16_t)i;
             s.group_start[g] = (uint16_t)((before & 0xffff) + c);
         }
-        before += n[j] + ((n[j] + kCols - 1) / kCols << 16);
+        before += n[j] + (((n[j] + kCols - 1) / kCols) << 16);
         cut |= n[j] > kCols;
     }
     if (tid == 0) {
         s.num_pairs = total & 0xffff;
         s.num_groups = total >> 16;
+        s.repeated = repeated;
     }
     cut = __syncthreads_or(cut);
 #pragma unroll
-    for (int j = 0; j < kMaxPairs / kThreads; ++j)
-        if (e[j] >= 0) s.pair[atomicAdd(&s.start[e[j]], 1)] = (uint16_t)(j * kThreads + tid);
+    for (int j = 0; j < kOwn; ++j)
+        if (e[j] >= 0) s.pair[atomicAdd(start + e[j], 1)] = (uint16_t)(j * kThreads + tid);
     __syncthreads();
     if (!cut) return;
-    int to[kMaxPairs / kThreads];
+    int to[kOwn];
 #pragma unroll
-    for (int j = 0; j < kMaxPairs / kThreads; ++j) {
+    for (int j = 0; j < kOwn; ++j) {
         if (e[j] < 0) continue;
-        const int begin = e[j] > 0 ? s.start[e[j] - 1] : 0, stop = s.start[e[j]];  // (each has moved on to the end of its own)
+        const int begin = e[j] > 0 ? start[e[j] - 1] : 0, stop = start[e[j]];  // (each has moved on to the end of its own)
         to[j] = begin;
         for (int i = begin; i < stop; ++i) to[j] += s.pair[i] < j * kThreads + tid;
     }
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < kMaxPairs / kThreads; ++j)
+    for (int j = 0; j < kOwn; ++j)
         if (e[j] >= 0) s.pair[to[j]] = (uint16_t)(j * kThreads + tid);
     __syncthreads();
 }
 
-// kUp: gate and up rows against x; otherwise W2 rows against h.
-template <bool kUp, bool kFp8>
-__global__ void __launch_bounds__(kThreads, 2) few_kernel(const __grid_constant__ CUtensorMap map, const FewParams p) {
-    extern __shared__ uint8_t raw[];
-    Smem& s = *reinterpret_cast<Smem*>(raw + ((1024 - (smem_u32(raw) & 1023)) & 1023));
-    const FewTokensArgs& a = p.a;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    constexpr int kBoxK = kFp8 ? 128 : 64;
-    const int depth = kUp ? a.hidden : a.inter;                           // the reduction
-    const int blocks = kUp ? (a.inter + 15) / 16 : (a.hidden + 31) / 32;  // units of one group
-    const int boxes = (depth + kBoxK - 1) / kBoxK;
-
-    if (tid < kWarps * kStages) mbar_init(&s.full[0][0] + tid, 1);
-    if (tid == 0) {
+__device__ __forceinline__ void start_barriers(const CUtensorMap* map, Plan& s) {
+    if (threadIdx.x < kWarps * kMostStages) mbar_init(&s.full[0][0] + threadIdx.x, 1);
+    if (threadIdx.x == 0) {
         s.abort = 0;
-        tma_prefetch_desc(&map);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tma_prefetch_desc(map);
     }
-    // What the second launch plans from was there before the first one began (which has waited for it); only h has to be waited for.
-    if constexpr (kUp) {
-        pdl_wait_predecessor();
-        pdl_release_successor();
-    }
-    plan(a, s);
-    const int groups = s.num_groups, units = groups * blocks;
-    // Units of this CTA. First launch: dealt out, group by group. Second: neighbours, result rows by result rows, so that a CTA has a part in few of them.
-    const int first = kUp ? (int)blockIdx.x : (int)((long long)blockIdx.x * units / gridDim.x);
-    const int end = kUp ? units : (int)((long long)(blockIdx.x + 1) * units / gridDim.x);
-    const int step = kUp ? (int)gridDim.x : 1;
-    auto group_of = [&](int u) { return kUp ? u / blocks : u % groups; };
-    auto block_of = [&](int u) { return kUp ? u % blocks : u / groups; };
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 
-    // ---- this warp's boxes, in order: number `warp` of the CTA's first unit and every eighth from there
-    int pu = first, pj = warp, issued = 0;
-    auto issue = [&] {  // the warp's next box, if there is one
-        while (pj >= boxes) {
-            pj -= boxes;
-            pu += step;
+// A warp's ring of boxes.
+struct Ring {
+    uint32_t at, bars;
+    int stages, fill, slot, parity, flying;
+    bool alive;
+    __device__ __forceinline__ Ring(uint8_t* smem, Plan& s, int warp, int stages_) {
+        at = smem_u32(smem) + warp * stages_ * kBoxBytes;
+        bars = smem_u32(s.full[warp]);
+        stages = stages_;
+        fill = slot = parity = flying = 0;
+        alive = true;
+    }
+    __device__ __forceinline__ uint32_t fill_at() const { return at + fill * kBoxBytes; }
+    __device__ __forceinline__ uint32_t fill_bar() const { return bars + fill * 8; }
+    __device__ __forceinline__ void filled() {
+        fill = fill + 1 == stages ? 0 : fill + 1;
+        ++flying;
+    }
+    // Waits for the next box; its place.
+    __device__ __forceinline__ uint32_t next(uint64_t* full, int* abort, long long limit) {
+        alive = __all_sync(0xffffffffu, mbar_wait(full + slot, parity, abort, limit)) && alive;
+        const uint32_t box = at + slot * kBoxBytes;
+        if (++slot == stages) {
+            slot = 0;
+            parity ^= 1;
         }
-        if (pu >= end) return;
-        if (lane == 0) {
-            const int slot = issued % kStages;
-            const uint32_t bar = smem_u32(&s.full[warp][slot]);
-            mbar_expect_tx_at(bar, kBoxBytes);
-            const int e = s.group_expert[group_of(pu)];
-            tma_load_box(&map, bar, smem_u32(s.ring[warp][slot]), pj * kBoxK, block_of(pu) * (kUp ? 16 : 32), 0, e, kUp);
+        --flying;
+        return box;
+    }
+    // A copy did not come: waits for those in flight and says so.
+    __device__ __forceinline__ void give_up(uint64_t* full, int* error_flag, long long limit) {
+        for (; flying > 0; --flying) {
+            const long long t0 = clock64();
+            while (!mbar_try_wait(full + slot, parity) && clock64() - t0 < limit) {}
+            if (++slot == stages) {
+                slot = 0;
+                parity ^= 1;
+            }
         }
-        ++issued;
-        pj += kWarps;
+        if (lane_id() == 0 && error_flag != nullptr) atomicExch(error_flag, 1);
+    }
+};
+
+// A box in registers: [16 rows][upper or lower eight][half of the 128 bytes]
+__device__ __forceinline__ void read_box(uint32_t box, int row, int t, int4 (&w)[2][2][2]) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) w[m][r][c] = lds128(box + (m * 16 + r * 8 + row) * 128 + (((c * 4 + t) ^ row) << 4));
+}
+// Sixteen rows' products: bf16 weights; e4m3 weights as bf16 or fp16. `b`: pieces of eight activations per lane.
+__device__ __forceinline__ void multiply(float (&d)[4], const int4& upper, const int4& lower, const int4& b) {
+    mma16<false>(d, upper.x, lower.x, upper.y, lower.y, b.x, b.y);
+    mma16<false>(d, upper.z, lower.z, upper.w, lower.w, b.z, b.w);
+}
+template <bool kHalf>
+__device__ __forceinline__ void multiply_fp8(float (&d)[4], const int4& upper, const int4& lower, const int4 (&b)[2]) {
+    const uint32_t u[4] = {(uint32_t)upper.x, (uint32_t)upper.y, (uint32_t)upper.z, (uint32_t)upper.w};
+    const uint32_t l[4] = {(uint32_t)lower.x, (uint32_t)lower.y, (uint32_t)lower.z, (uint32_t)lower.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint32_t a0, a1, a2, a3;
+        if constexpr (kHalf) {
+            e4m3x4_to_half(u[q], a0, a2);
+            e4m3x4_to_half(l[q], a1, a3);
+        } else {
+            e4m3x4_to_bf16(u[q], a0, a2);
+            e4m3x4_to_bf16(l[q], a1, a3);
+        }
+        mma16<kHalf>(d, a0, a1, a2, a3, (q & 1) ? b[q / 2].z : b[q / 2].x, (q & 1) ? b[q / 2].w : b[q / 2].y);
+    }
+}
+// Fragment row g of eight is row_of(g): neighbours in g are four rows apart, on other banks.
+__device__ __forceinline__ int row_of(int g) { return (g >> 1) | ((g & 1) << 2); }
+__device__ __forceinline__ int lane_row_of(int r) { return ((r & 3) << 1) | (r >> 2); }  // its inverse
+
+// ---- first launch: gate and up rows against x ---------------------------------------------------------------------------------------------
+template <bool kFp8>
+__global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_constant__ CUtensorMap map, const FewParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const FewTokensArgs& a = p.a;
+    constexpr int kStages = stages_for(true, 1), kBoxK = kFp8 ? 128 : 64;
+    float4(*red)[2][32] = reinterpret_cast<float4(*)[2][32]>(smem + ring_bytes(kStages));
+    Plan& s = *reinterpret_cast<Plan*>(smem + ring_bytes(kStages) + sum_bytes(true, 1));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, row = row_of(g);
+    const int blocks = (a.inter + 15) / 16, boxes = (a.hidden + kBoxK - 1) / kBoxK;  // units of one group, boxes of a unit
+
+    start_barriers(&map, s);
+    pdl_wait_predecessor();
+    pdl_release_successor();
+    make_plan(a, s, reinterpret_cast<int*>(red));
+    const int groups = s.num_groups, units = groups * blocks;
+    // Units are dealt to the teams in turn, group by group, those of an SM last.
+    const int team = warp / kTeamWarps, member = warp % kTeamWarps, step = kWarps / kTeamWarps * (int)gridDim.x;
+    struct Place {
+        int u, group, block;
+    };
+    const int step_group = step / blocks, step_block = step % blocks;
+    auto advance = [&](Place& at) {
+        at.u += step;
+        at.group += step_group;
+        at.block += step_block;
+        if (at.block >= blocks) {
+            at.block -= blocks;
+            ++at.group;
+        }
+    };
+    const int first = team * (int)gridDim.x + (int)blockIdx.x;
+    Place now{first, first / blocks, first % blocks}, ahead = now;
+    Ring ring(smem, s, warp, kStages);
+    int ahead_j = member;  // the warp's boxes: from `member` of the team's first unit on in steps of the team's size
+    auto issue = [&] {
+        while (ahead_j >= boxes) {
+            ahead_j -= boxes;
+            advance(ahead);
+        }
+        if (ahead.u >= units) {
+            ahead_j = 0;
+            return;
+        }
+        const int e = s.group_expert[ahead.group];
+        if (elect_one()) {
+            mbar_expect_tx_at(ring.fill_bar(), kBoxBytes);
+            tma_load_box(&map, ring.fill_bar(), ring.fill_at(), ahead_j * kBoxK, ahead.block * 16, 0, e);
+        }
+        ring.filled();
+        ahead_j += kTeamWarps;
     };
     for (int i = 0; i < kStages; ++i) issue();
-    if constexpr (!kUp) {
-        pdl_wait_predecessor();
-        pdl_release_successor();
-    } else if (blockIdx.x == 0) {
-        for (int i = tid; i < (a.hidden + 31) / 32; i += kThreads) p.finished[i] = 0;
-    }
+    auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kTeamWarps * 32) : "memory"); };
 
-    const int row = (g >> 1) | ((g & 1) << 2);  // of a fragment's eight rows: neighbours in g are four rows apart, on other banks
-    const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(a.h);
-    const long long plane = (long long)a.tokens * a.topk * a.inter;  // from a rounding to its remainder
-    int used = 0, j = warp;
-    for (int u = first; u < end; u += step) {
-        const int group = group_of(u), block = block_of(u), e = s.group_expert[group], at = s.group_start[group];
-        const int stop = group + 1 < groups ? s.group_start[group + 1] : s.num_pairs, n = stop - at;
+    int j = member;
+    for (; now.u < units; advance(now)) {
+        const int block = now.block, at = s.group_start[now.group], n = (now.group + 1 < groups ? s.group_start[now.group + 1] : s.num_pairs) - at;
         const int mine = g < n ? s.pair[at + g] : -1;  // this lane's column
-        const __nv_bfloat16* b_row = mine < 0 ? nullptr
-                                     : kUp    ? reinterpret_cast<const __nv_bfloat16*>(a.x) + (mine / a.topk) * a.x_stride
-                                              : h + (long long)mine * a.inter;
+        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (mine / a.topk) * a.x_stride;
+        const int blocks_k = a.hidden / 128;
+        const float* scales = kFp8 ? a.s13 + ((long long)s.group_expert[now.group] * (2 * a.inter / 128) + block * 16 / 128) * blocks_k : nullptr;
         float acc[2][4] = {};
-        for (; j < boxes; j += kWarps) {
-            constexpr int kPieces = kFp8 ? 4 : 2;  // of 16 bytes of activations per lane
-            int4 b[kPieces], b_lo[kPieces];
+        for (; j < boxes; j += kTeamWarps) {
+            constexpr int kPieces = kFp8 ? 4 : 2;
+            int4 b[kPieces], w[2][2][2];
 #pragma unroll
             for (int i = 0; i < kPieces; ++i) {
                 const int k = j * kBoxK + (kFp8 ? (i >> 1) * 64 + t * 16 + (i & 1) * 8 : i * 32 + t * 8);
-                const bool in = mine >= 0 && k < depth;
-                b[i] = in ? *reinterpret_cast<const int4*>(b_row + k) : make_int4(0, 0, 0, 0);
-                if constexpr (!kUp) b_lo[i] = in ? *reinterpret_cast<const int4*>(b_row + plane + k) : make_int4(0, 0, 0, 0);
+                b[i] = mine >= 0 && k < a.hidden ? *reinterpret_cast<const int4*>(x + k) : make_int4(0, 0, 0, 0);
             }
             float scale[2] = {1.f, 1.f};
             if constexpr (kFp8) {
-                const int kb = depth / 128;
-                if constexpr (kUp) {
-                    const float* sc = a.s13 + ((long long)e * (2 * a.inter / 128) + block * 16 / 128) * kb + j;
-                    scale[0] = __ldg(sc);
-                    scale[1] = __ldg(sc + (long long)(a.inter / 128) * kb);
-                } else {
-                    scale[0] = scale[1] = __ldg(a.s2 + ((long long)e * (a.hidden / 128) + block * 32 / 128) * kb + j);
-                }
+                scale[0] = __ldg(scales + j);
+                scale[1] = __ldg(scales + (long long)(a.inter / 128) * blocks_k + j);
             }
-            const int slot = used % kStages;
-            mbar_wait(&s.full[warp][slot], (used / kStages) & 1, &s.abort, p.limit);
-            const uint32_t base = smem_u32(s.ring[warp][slot]);
-            int4 w[2][2][2];  // [16 rows][upper or lower eight][half of the 128 bytes]
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int r = 0; r < 2; ++r)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) w[m][r][c] = lds128(base + (m * 16 + r * 8 + row) * 128 + (((c * 4 + t) ^ row) << 4));
-            ++used;
+            read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
             __syncwarp();
-            if (!s.abort) issue();
+            if (ring.alive) issue();
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                float part[4] = {};
-                float(&d)[4] = kFp8 ? part : acc[m];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t w0[4] = {(uint32_t)w[m][0][c].x, (uint32_t)w[m][0][c].y, (uint32_t)w[m][0][c].z, (uint32_t)w[m][0][c].w};
-                    const uint32_t w1[4] = {(uint32_t)w[m][1][c].x, (uint32_t)w[m][1][c].y, (uint32_t)w[m][1][c].z, (uint32_t)w[m][1][c].w};
-                    if constexpr (kFp8) {
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            uint32_t a0, a1, a2, a3;
-                            e4m3x4_to_bf16(w0[q], a0, a2);
-                            e4m3x4_to_bf16(w1[q], a1, a3);
-                            const int4 &v = b[c * 2 + q / 2], &lo = b_lo[c * 2 + q / 2];
-                            mma_bf16(d, a0, a1, a2, a3, (q & 1) ? v.z : v.x, (q & 1) ? v.w : v.y);
-                            if constexpr (!kUp) mma_bf16(d, a0, a1, a2, a3, (q & 1) ? lo.z : lo.x, (q & 1) ? lo.w : lo.y);
-                        }
-                    } else {
-                        mma_bf16(d, w0[0], w1[0], w0[1], w1[1], b[c].x, b[c].y);
-                        mma_bf16(d, w0[2], w1[2], w0[3], w1[3], b[c].z, b[c].w);
-                        if constexpr (!kUp) {
-                            mma_bf16(d, w0[0], w1[0], w0[1], w1[1], b_lo[c].x, b_lo[c].y);
-                            mma_bf16(d, w0[2], w1[2], w0[3], w1[3], b_lo[c].z, b_lo[c].w);
-                        }
-                    }
-                }
                 if constexpr (kFp8) {
+                    float part[4] = {};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const int4 two[2] = {b[(2 * c) % kPieces], b[(2 * c + 1) % kPieces]};
+                        multiply_fp8<false>(part, w[m][0][c], w[m][1][c], two);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[m], part[i], acc[m][i]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) multiply(acc[m], w[m][0][c], w[m][1][c], b[c]);
                 }
             }
         }
         j -= boxes;
-        // ---- the warps' partial sums: fragment place (lane, i) = row (lane / 4 by `row`, + 8 for i >= 2), column 2 (lane % 4) + i % 2
+        // the warps' partial sums: place (lane, i) of a fragment is row row_of(lane / 4), + 8 for i >= 2, column 2 (lane % 4) + i % 2
 #pragma unroll
-        for (int m = 0; m < 2; ++m) s.red[warp][m][lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
-        __syncthreads();
-        auto sum = [&](int m, int r, int c) {
-            const int from = ((((r & 3) << 1) | ((r >> 2) & 1)) * 4 + (c >> 1)) * 4 + ((r >> 3) << 1) + (c & 1);
-            float v = 0.f;
+        for (int m = 0; m < 2; ++m) red[warp][m][lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+        meet();
+        for (int o = member * 32 + lane; o < 16 * n; o += kTeamWarps * 32) {
+            const int r = o & 15, c = o >> 4, i = block * 16 + r, from = (lane_row_of(r & 7) * 4 + (c >> 1)) * 4 + ((r >> 3) << 1) + (c & 1);
+            float gate = 0.f, up = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) v += reinterpret_cast<const float*>(s.red[w][m])[from];
-            return v;
-        };
-        if constexpr (kUp) {
-            const int r = tid & 15, c = tid >> 4, i = block * 16 + r;
-            if (c < n && i < a.inter) {
-                const int q = s.pair[at + c];
-                const float v = silu(sum(0, r, c)) * sum(1, r, c) * a.weights[q];
+            for (int w = 0; w < kTeamWarps; ++w) {
+                gate += reinterpret_cast<const float*>(red[team * kTeamWarps + w][0])[from];
+                up += reinterpret_cast<const float*>(red[team * kTeamWarps + w][1])[from];
+            }
+            const int q = s.pair[at + c];
+            float weight = a.weights[q];
+            if (s.repeated)
+                for (int k = q % a.topk + 1, z = q + 1; k < a.topk; ++k, ++z)
+                    if (a.idx[z] == a.idx[q]) weight += a.weights[z];
+            const float v = silu(gate) * up * weight;
+            const long long to = (long long)q * a.inter + i;
+            if constexpr (kFp8) {
+                // sixteen lanes have the sixteen values of a scale: the power of two at or below the largest
+                float most = fabsf(v);
+#pragma unroll
+                for (int x16 = 8; x16 > 0; x16 >>= 1) most = fmaxf(most, __shfl_xor_sync((lane & 16) ? 0xffff0000u : 0xffffu, most, x16));
+                const int field = most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23), 1), 253) : 127;
+                reinterpret_cast<__half*>(p.h)[to] = __float2half(v * __uint_as_float((uint32_t)(254 - field) << 23));
+                if (r == 0) p.h_scale[to / 16] = __uint_as_float((uint32_t)field << 23);
+            } else if (i < a.inter) {
                 const __nv_bfloat16 hi = __float2bfloat16(v);
-                __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(a.h) + (long long)q * a.inter + i;
-                to[0] = hi;
-                to[plane] = __float2bfloat16(v - __bfloat162float(hi));
+                reinterpret_cast<__nv_bfloat16*>(p.h)[to] = hi;
+                reinterpret_cast<__nv_bfloat16*>(p.h)[to + (long long)a.tokens * a.topk * a.inter] = __float2bfloat16(v - __bfloat162float(hi));
             }
-            __syncthreads();
+        }
+        meet();
+    }
+    if (!ring.alive) ring.give_up(s.full[warp], a.error_flag, p.limit);
+}
+
+// ---- second launch: W2 rows against h ---------------------------------------------------------------------------------------------------
+template <bool kFp8>
+__global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_constant__ CUtensorMap map, const FewParams p) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const FewTokensArgs& a = p.a;
+    constexpr int kBoxK = kFp8 ? 128 : 64;
+    const int stages = stages_for(false, a.tokens);
+    float* sums = reinterpret_cast<float*>(smem + ring_bytes(stages));
+    Plan& s = *reinterpret_cast<Plan*>(smem + ring_bytes(stages) + sum_bytes(false, a.tokens));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3, row = row_of(g);
+    const int tile = (int)blockIdx.x / p.cluster, rank = (int)blockIdx.x % p.cluster, boxes = (a.inter + kBoxK - 1) / kBoxK;
+
+    start_barriers(&map, s);
+    // What this launch plans from was there before the first one began (which has waited for it); only h has to be waited for.
+    make_plan(a, s, reinterpret_cast<int*>(sums));
+    const int groups = s.num_groups;
+    const long long all = (long long)groups * boxes;
+    const int end = (int)(all * (rank + 1) / p.cluster), first = (int)(all * rank / p.cluster) + warp;  // this warp's boxes: every eighth from `first`, the groups' one after the other
+    struct Place {
+        int b, group, j;
+    };
+    auto advance = [&](Place& at) {
+        at.b += kWarps;
+        at.j += kWarps;
+        while (at.j >= boxes) {
+            at.j -= boxes;
+            ++at.group;
+        }
+    };
+    Place now{first, first / boxes, first % boxes}, ahead = now;
+    Ring ring(smem, s, warp, stages);
+    auto issue = [&] {
+        if (ahead.b >= end) return;
+        const int e = s.group_expert[ahead.group];
+        if (elect_one()) {
+            mbar_expect_tx_at(ring.fill_bar(), kBoxBytes);
+            tma_load_box(&map, ring.fill_bar(), ring.fill_at(), ahead.j * kBoxK, tile * kBoxRows, e);
+        }
+        ring.filled();
+        advance(ahead);
+    };
+    for (int i = 0; i < stages; ++i) issue();
+    // this warp's sums, [tokens][32 rows], the rows of a token turned by 8 per token so that four tokens' fragments are on different banks
+    float* mine_sums = sums + warp * a.tokens * kBoxRows;
+    for (int i = lane; i < a.tokens * kBoxRows; i += 32) mine_sums[i] = 0.f;
+    pdl_wait_predecessor();
+    pdl_release_successor();
+
+    float acc[2][4] = {};
+    int group = -1, at = 0, n = 0, mine = -1;
+    auto flush = [&] {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (2 * t + i >= n) continue;
+            const int token = s.pair[at + 2 * t + i] / a.topk;
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    mine_sums[token * kBoxRows + ((m * 16 + r * 8 + row + 8 * token) & 31)] += acc[m][2 * r + i];
+                    acc[m][2 * r + i] = 0.f;
+                }
+        }
+    };
+    const float* scales = nullptr;
+    for (; now.b < end; advance(now)) {
+        if (now.group != group) {
+            if (group >= 0) flush();
+            group = now.group;
+            at = s.group_start[group];
+            n = (group + 1 < groups ? s.group_start[group + 1] : s.num_pairs) - at;
+            mine = g < n ? s.pair[at + g] : -1;
+            if constexpr (kFp8) scales = a.s2 + ((long long)s.group_expert[group] * (a.hidden / 128) + tile * kBoxRows / 128) * (a.inter / 128);
+        }
+        int4 w[2][2][2];
+        if constexpr (kFp8) {
+            int4 b[4];
+            float hs[2] = {1.f, 1.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = make_int4(0, 0, 0, 0);
+            const float scale = __ldg(scales + now.j);
+            if (mine >= 0) {
+                const int4* h = reinterpret_cast<const int4*>(reinterpret_cast<const __half*>(p.h) + (long long)mine * a.inter + now.j * kBoxK + t * 16);
+                b[0] = h[0], b[1] = h[1], b[2] = h[8], b[3] = h[9];
+                const float* f = p.h_scale + (long long)mine * (a.inter / 16) + now.j * 8 + t;
+                hs[0] = f[0], hs[1] = f[4];
+            }
+            read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
+            __syncwarp();
+            if (ring.alive) issue();
+            // one power of two for the box's 128 values of a column: the largest of its eight
+            float top = fmaxf(hs[0], hs[1]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float under = __uint_as_float((254u << 23) - __float_as_uint(top));
+            const __half2 by[2] = {__float2half2_rn(hs[0] * under), __float2half2_rn(hs[1] * under)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                b[i] = make_int4((int)scale_half2(b[i].x, by[i / 2]), (int)scale_half2(b[i].y, by[i / 2]), (int)scale_half2(b[i].z, by[i / 2]), (int)scale_half2(b[i].w, by[i / 2]));
+            const float col[2] = {scale * __shfl_sync(0xffffffffu, top, 8 * t), scale * __shfl_sync(0xffffffffu, top, 8 * t + 4)};  // columns 2 t and 2 t + 1
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                float part[4] = {};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int4 two[2] = {b[2 * c], b[2 * c + 1]};
+                    multiply_fp8<true>(part, w[m][0][c], w[m][1][c], two);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(col[i & 1], part[i], acc[m][i]);
+            }
         } else {
-            const int r = tid & 31, c = tid >> 5, i = block * 32 + r;
-            if (c < n && i < a.hidden) p.y[(long long)s.pair[at + c] * a.hidden + i] = sum(r >> 4, r & 15, c);
-            __syncthreads();
-            // the end of this CTA's part in these result rows
-            if (u + 1 >= end || block_of(u + 1) != block) {
-                const int begun = max(first, block * groups);
-                if (tid == 0) {
-                    fence_acq_rel_gpu();
-                    s.last = atomicAdd(p.finished + block, u + 1 - begun) + u + 1 - begun == groups;
-                    fence_acq_rel_gpu();
-                }
-                __syncthreads();
-                if (s.last) {
-                    for (int o = tid; o < a.tokens * 32; o += kThreads) {
-                        const int tok = o >> 5, col = block * 32 + (o & 31);
-                        if (col >= a.hidden) continue;
-                        float v = 0.f;
-                        for (int k = 0; k < a.topk; ++k) {
-                            const int q = tok * a.topk + k;
-                            if (local_expert(a, a.idx[q]) >= 0) v += __ldcg(p.y + (long long)q * a.hidden + col);
-                        }
-                        reinterpret_cast<__nv_bfloat16*>(a.out)[(long long)tok * a.hidden + col] = __float2bfloat16(v);
-                    }
-                }
-                __syncthreads();
+            int4 b[2][2];  // [half of the box][rounding, remainder]
+            const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(p.h) + (long long)mine * a.inter;
+            const long long plane = (long long)a.tokens * a.topk * a.inter;
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int k = now.j * kBoxK + c * 32 + t * 8;
+                const bool in = mine >= 0 && k < a.inter;
+                b[c][0] = in ? *reinterpret_cast<const int4*>(h + k) : make_int4(0, 0, 0, 0);
+                b[c][1] = in ? *reinterpret_cast<const int4*>(h + plane + k) : make_int4(0, 0, 0, 0);
             }
+            read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
+            __syncwarp();
+            if (ring.alive) issue();
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    multiply(acc[m], w[m][0][c], w[m][1][c], b[c][0]);
+                    multiply(acc[m], w[m][0][c], w[m][1][c], b[c][1]);
+                }
         }
     }
-    if constexpr (!kUp) {
-        if (groups == 0)  // nobody's expert is here
-            for (long long i = (long long)blockIdx.x * kThreads + tid; i < (long long)a.tokens * a.hidden; i += (long long)gridDim.x * kThreads)
-                reinterpret_cast<__nv_bfloat16*>(a.out)[i] = __float2bfloat16(0.f);
+    if (group >= 0) flush();
+    if (!ring.alive) ring.give_up(s.full[warp], a.error_flag, p.limit);
+    __syncthreads();
+    // the warps' sums, in order, and then the cluster's
+    const int outputs = a.tokens * kBoxRows;
+    auto store = [&](int o, float v) {
+        const int token = o / kBoxRows, i = tile * kBoxRows + ((o - 8 * token) & 31);
+        if (i < a.hidden) reinterpret_cast<__nv_bfloat16*>(a.out)[(long long)token * a.hidden + i] = __float2bfloat16(v);
+    };
+    for (int o = tid; o < outputs; o += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += sums[w * outputs + o];
+        if (p.cluster == 1)
+            store(o, v);
+        else
+            sums[o] = v;  // (this thread's alone until the cluster meets)
     }
-    if (s.abort) {  // a copy did not come: wait for those in flight, then say so
-        for (; used < issued; ++used) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(&s.full[warp][used % kStages], (used / kStages) & 1) && clock64() - t0 < p.limit) {}
-        }
-        if (tid == 0 && p.error_flag != nullptr) atomicExch(p.error_flag, 1);
+    if (p.cluster == 1) return;
+    cluster_sync();
+    for (int o = rank * kThreads + tid; o < outputs; o += p.cluster * kThreads) {
+        float v = 0.f;
+        for (int c = 0; c < p.cluster; ++c) v += ld_cluster_f32(sums + o, c);
+        store(o, v);
     }
+    cluster_sync();  // (nobody leaves while its sums are read)
 }
 
 // The weights as boxes of 128 bytes of neighbouring rows: [L, 2, I, H] in boxes of 16 gate and 16 up rows, [L, H, I] in boxes of 32 rows.
-bool make_weight_map(CUtensorMap* map, const void* ptr, bool fp8, uint64_t experts, uint64_t halves, uint64_t rows, uint64_t depth) {
+bool make_weight_map(CUtensorMap* map, const void* ptr, bool fp8, bool up, uint64_t experts, uint64_t rows, uint64_t depth) {
     EncodeFn fn = get_encode_fn();
     if (fn == nullptr) return false;
     const uint64_t esz = fp8 ? 1 : 2;
-    const bool up = halves == 2;
-    const cuuint64_t dims[4] = {depth, rows, up ? halves : experts, experts};
-    const cuuint64_t strides[3] = {depth * esz, rows * depth * esz, halves * rows * depth * esz};
+    const cuuint64_t dims[4] = {depth, rows, up ? 2 : experts, experts};
+    const cuuint64_t strides[3] = {depth * esz, rows * depth * esz, 2 * rows * depth * esz};
     const cuuint32_t box[4] = {(cuuint32_t)(128 / esz), up ? 16u : 32u, up ? 2u : 1u, 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     return fn(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, up ? 4 : 3, const_cast<void*>(ptr), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
-static_assert(2 * (kSmemBytes + 1024) <= 228 * 1024, "two CTAs share an SM");
-
-template <bool kUp, bool kFp8>
-cudaError_t launch_half(const FewParams& p, int ctas, cudaStream_t stream) {
+template <bool kFp8>
+cudaError_t launch_both(FewParams& p, int num_sms, cudaStream_t stream) {
     const FewTokensArgs& a = p.a;
-    CUtensorMap map;
-    if (!make_weight_map(&map, kUp ? a.w13 : a.w2, kFp8, a.experts, kUp ? 2 : 1, kUp ? a.inter : a.hidden, kUp ? a.hidden : a.inter)) return cudaErrorInvalidValue;
-    const cudaError_t e = cudaFuncSetAttribute(few_kernel<kUp, kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes);
+    CUtensorMap up, down;
+    if (!make_weight_map(&up, a.w13, kFp8, true, a.experts, a.inter, a.hidden) || !make_weight_map(&down, a.w2, kFp8, false, a.experts, a.hidden, a.inter))
+        return cudaErrorInvalidValue;
+    const size_t up_smem = smem_bytes(true, 1), down_smem = smem_bytes(false, a.tokens);
+    cudaError_t e = cudaFuncSetAttribute(few_up_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)up_smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_down_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_smem);
+    if (e == cudaSuccess) e = launch_dependent(few_up_kernel<kFp8>, dim3((unsigned)(2 * num_sms)), kThreads, up_smem, stream, up, p);
     if (e != cudaSuccess) return e;
-    return launch_dependent(few_kernel<kUp, kFp8>, dim3((unsigned)ctas), kThreads, kSmemBytes, stream, map, p);
+    // as many CTAs as two per SM hold
+    const int tiles = (a.hidden + kBoxRows - 1) / kBoxRows;
+    p.cluster = 1;
+    while (p.cluster < 8 && tiles * p.cluster * 2 <= 2 * num_sms) p.cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * p.cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = down_smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, few_down_kernel<kFp8>, down, p);
 }
 
-size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
-size_t h_bytes(const FewTokensArgs& a) { return aligned((size_t)2 * a.tokens * a.topk * a.inter * 2); }
-size_t y_bytes(const FewTokensArgs& a) { return aligned((size_t)a.tokens * a.topk * a.hidden * 4); }
+size_t h_bytes(const FewTokensArgs& a) { return ((size_t)a.tokens * a.topk * a.inter * (a.fp8 ? 2 : 4) + 255) / 256 * 256; }
 
 }  // namespace
 
-size_t few_tokens_scratch(const FewTokensArgs& a) { return h_bytes(a) + y_bytes(a) + aligned((size_t)(a.hidden + 31) / 32 * 4); }
+size_t few_tokens_scratch(const FewTokensArgs& a) { return h_bytes(a) + (a.fp8 ? (size_t)a.tokens * a.topk * (a.inter / 16) * 4 : 0); }
 
-cudaError_t launch_few_tokens(const FewTokensArgs& args, int num_sms, cudaStream_t stream) {
-    if (args.tokens <= 0) return cudaSuccess;
-    const int unit = args.fp8 ? 128 : 8;
-    if (args.tokens > kFewMaxTokens || args.topk < 1 || args.topk > kFewMaxTopk || args.experts < 1 || args.experts > kFewMaxExperts || args.hidden <= 0 ||
-        args.hidden % unit != 0 || args.inter <= 0 || args.inter % unit != 0)
+cudaError_t launch_few_tokens(const FewTokensArgs& a, int num_sms, cudaStream_t stream) {
+    if (a.tokens <= 0) return cudaSuccess;
+    const int unit = a.fp8 ? 128 : 8;
+    if (a.tokens > kFewMaxTokens || a.topk < 1 || a.topk > kFewMaxTopk || a.experts < 1 || a.experts > kFewMaxExperts || a.hidden <= 0 || a.hidden % unit != 0 ||
+        a.inter <= 0 || a.inter % unit != 0)
         return cudaErrorInvalidValue;
     FewParams p{};
-    p.a = args;
-    p.a.h = args.scratch;
-    p.y = reinterpret_cast<float*>(static_cast<char*>(args.scratch) + h_bytes(args));
-    p.finished = reinterpret_cast<int*>(static_cast<char*>(args.scratch) + h_bytes(args) + y_bytes(args));
-    p.error_flag = args.error_flag;
-    p.limit = args.wait_limit;
-    const cudaError_t e = args.fp8 ? launch_half<true, true>(p, 2 * num_sms, stream) : launch_half<true, false>(p, 2 * num_sms, stream);
-    if (e != cudaSuccess) return e;
-    return args.fp8 ? launch_half<false, true>(p, 2 * num_sms, stream) : launch_half<false, false>(p, 2 * num_sms, stream);
+    p.a = a;
+    p.h = a.scratch;
+    p.h_scale = reinterpret_cast<float*>(static_cast<char*>(a.scratch) + h_bytes(a));
+    p.limit = a.wait_limit;
+    return a.fp8 ? launch_both<true>(p, num_sms, stream) : launch_both<false>(p, num_sms, stream);
 }
 
 }  // namespace dx
