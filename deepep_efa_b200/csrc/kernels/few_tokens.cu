@@ -18,9 +18,9 @@
 // meet at the end, in a fixed order. So nothing is exchanged through memory but h, and no result depends on an order of arrival. The second launch begins
 // while the first one ends (programmatic dependent launch): it plans, fills its rings with weights, and only then waits for h.
 //
-// Types: e4m3 becomes bf16 (first launch) or fp16 (second) in registers, exactly, and each 128 x 128 block's sum is scaled in fp32. h has more bits than bf16, so that its rounding
-// is small beside that of the result: next to bf16 weights two bf16 numbers, a rounding and its remainder, whose products go to the same accumulators; next to
-// e4m3 weights fp16 with a power of two per 16 values.
+// Types: e4m3 becomes fp16 in registers, exactly and with one instruction per pair (bf16 takes four: 8 tokens, FP8, us XXX), and each 128 x 128 block's sum is scaled in
+// fp32. Next to it activations are fp16 times a power of two per 128 of them. h has more bits than bf16, so that its rounding is small beside that of the result: next
+// to bf16 weights two bf16 numbers, a rounding and its remainder, whose products go to the same accumulators; next to e4m3 weights fp16 with a power of two per 16 values.
 #include <cuda.h>
 
 #include <cuda_fp16.h>
@@ -106,18 +106,39 @@ __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, u
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Four e4m3 numbers as two pairs (bytes 0 and 1, bytes 2 and 3) in fp16 or bf16, which hold each of them, NaN included.
+// Four e4m3 numbers as two pairs (bytes 0 and 1, bytes 2 and 3) in fp16, which holds each of them, NaN included.
 __device__ __forceinline__ void e4m3x4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
-__device__ __forceinline__ uint32_t half2_to_bf16x2(uint32_t v) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
-    return f2_to_bf16x2(f.x, f.y);
-}
-__device__ __forceinline__ void e4m3x4_to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    e4m3x4_to_half(w, lo, hi);
-    lo = half2_to_bf16x2(lo);
-    hi = half2_to_bf16x2(hi);
+// The activations of a box (32 of 128 per lane, those of a column in four neighbouring lanes) from bf16 to fp16 times `top`, the power of two at or below the column's largest
+// magnitude. Exact down to 2^-17 of that; what is smaller keeps an absolute error of 2^-25 of it.
+template <int N>
+__device__ __forceinline__ void to_half(int4 (&b)[N], float& top) {
+    __nv_bfloat162 most = __float2bfloat162_rn(0.f);
+    uint32_t v[N][4];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        v[i][0] = b[i].x, v[i][1] = b[i].y, v[i][2] = b[i].z, v[i][3] = b[i].w;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) most = __hmax2(most, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[i][q])));
+    }
+    float f = fmaxf(__low2float(most), __high2float(most));
+    f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 1));
+    f = fmaxf(f, __shfl_xor_sync(0xffffffffu, f, 2));
+    const uint32_t field = min(max(__float_as_uint(f) >> 23, 1u), 253u);
+    top = __uint_as_float(field << 23);
+    const uint32_t under = (254u - field) << 7, both = under | (under << 16);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const __nv_bfloat162 u = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&v[i][q]), *reinterpret_cast<const __nv_bfloat162*>(&both));
+            const float2 w = __bfloat1622float2(u);
+            const __half2 r = __floats2half2_rn(w.x, w.y);
+            v[i][q] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+        b[i] = make_int4((int)v[i][0], (int)v[i][1], (int)v[i][2], (int)v[i][3]);
+    }
 }
 __device__ __forceinline__ uint32_t scale_half2(uint32_t v, __half2 by) {
     const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), by);
@@ -269,26 +290,21 @@ __device__ __forceinline__ void read_box(uint32_t box, int row, int t, int4 (&w)
 #pragma unroll
             for (int c = 0; c < 2; ++c) w[m][r][c] = lds128(box + (m * 16 + r * 8 + row) * 128 + (((c * 4 + t) ^ row) << 4));
 }
-// Sixteen rows' products: bf16 weights; e4m3 weights as bf16 or fp16. `b`: pieces of eight activations per lane.
+// Sixteen rows' products with pieces of eight activations per lane: bf16 weights, e4m3 weights as fp16.
 __device__ __forceinline__ void multiply(float (&d)[4], const int4& upper, const int4& lower, const int4& b) {
     mma16<false>(d, upper.x, lower.x, upper.y, lower.y, b.x, b.y);
     mma16<false>(d, upper.z, lower.z, upper.w, lower.w, b.z, b.w);
 }
-template <bool kHalf>
-__device__ __forceinline__ void multiply_fp8(float (&d)[4], const int4& upper, const int4& lower, const int4 (&b)[2]) {
+__device__ __forceinline__ void multiply_fp8(float (&d)[4], const int4& upper, const int4& lower, const int4& b0, const int4& b1) {
     const uint32_t u[4] = {(uint32_t)upper.x, (uint32_t)upper.y, (uint32_t)upper.z, (uint32_t)upper.w};
     const uint32_t l[4] = {(uint32_t)lower.x, (uint32_t)lower.y, (uint32_t)lower.z, (uint32_t)lower.w};
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
         uint32_t a0, a1, a2, a3;
-        if constexpr (kHalf) {
-            e4m3x4_to_half(u[q], a0, a2);
-            e4m3x4_to_half(l[q], a1, a3);
-        } else {
-            e4m3x4_to_bf16(u[q], a0, a2);
-            e4m3x4_to_bf16(l[q], a1, a3);
-        }
-        mma16<kHalf>(d, a0, a1, a2, a3, (q & 1) ? b[q / 2].z : b[q / 2].x, (q & 1) ? b[q / 2].w : b[q / 2].y);
+        e4m3x4_to_half(u[q], a0, a2);
+        e4m3x4_to_half(l[q], a1, a3);
+        const int4& b = q < 2 ? b0 : b1;
+        mma16<true>(d, a0, a1, a2, a3, (q & 1) ? b.z : b.x, (q & 1) ? b.w : b.y);
     }
 }
 // Fragment row g of eight is row_of(g): neighbours in g are four rows apart, on other banks.
@@ -366,29 +382,31 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
                 const int k = j * kBoxK + (kFp8 ? (i >> 1) * 64 + t * 16 + (i & 1) * 8 : i * 32 + t * 8);
                 b[i] = mine >= 0 && k < a.hidden ? *reinterpret_cast<const int4*>(x + k) : make_int4(0, 0, 0, 0);
             }
-            float scale[2] = {1.f, 1.f};
             if constexpr (kFp8) {
-                scale[0] = __ldg(scales + j);
-                scale[1] = __ldg(scales + (long long)(a.inter / 128) * blocks_k + j);
-            }
-            read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
-            __syncwarp();
-            if (ring.alive) issue();
+                const float gate = __ldg(scales + j), up = __ldg(scales + (long long)(a.inter / 128) * blocks_k + j);
+                read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
+                __syncwarp();
+                if (ring.alive) issue();
+                float top;
+                to_half(b, top);
+                const float even = __shfl_sync(0xffffffffu, top, 8 * t), odd = __shfl_sync(0xffffffffu, top, 8 * t + 4);  // columns 2 t and 2 t + 1
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                if constexpr (kFp8) {
+                for (int m = 0; m < 2; ++m) {
                     float part[4] = {};
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int4 two[2] = {b[(2 * c) % kPieces], b[(2 * c + 1) % kPieces]};
-                        multiply_fp8<false>(part, w[m][0][c], w[m][1][c], two);
-                    }
+                    for (int c = 0; c < 2; ++c) multiply_fp8(part, w[m][0][c], w[m][1][c], b[(2 * c) % kPieces], b[(2 * c + 1) % kPieces]);
+                    const float scale = m == 0 ? gate : up;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale[m], part[i], acc[m][i]);
-                } else {
+                    for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(scale * ((i & 1) ? odd : even), part[i], acc[m][i]);
+                }
+            } else {
+                read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
+                __syncwarp();
+                if (ring.alive) issue();
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
                     for (int c = 0; c < 2; ++c) multiply(acc[m], w[m][0][c], w[m][1][c], b[c]);
-                }
             }
         }
         j -= boxes;
@@ -534,10 +552,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
             for (int m = 0; m < 2; ++m) {
                 float part[4] = {};
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int4 two[2] = {b[2 * c], b[2 * c + 1]};
-                    multiply_fp8<true>(part, w[m][0][c], w[m][1][c], two);
-                }
+                for (int c = 0; c < 2; ++c) multiply_fp8(part, w[m][0][c], w[m][1][c], b[2 * c], b[2 * c + 1]);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(col[i & 1], part[i], acc[m][i]);
             }
