@@ -44,7 +44,7 @@ constexpr int kTeamWarps = 4;  // warps that share a unit of the first launch
 
 // What a CTA plans by: the selections in the order of their experts, and groups of up to eight of one expert.
 struct Plan {
-    uint16_t pair[kMaxPairs];  // selection t * topk + k
+    uint16_t pair[kMaxPairs];  // selection k of token t: t << 5 | k
     uint16_t group_expert[kMaxPairs], group_start[kMaxPairs];
     uint64_t full[kWarps][kMostStages];
     int warp_sum[kWarps];
@@ -152,6 +152,7 @@ __device__ __forceinline__ void make_plan(const FewTokensArgs& a, Plan& s, int* 
     constexpr int kOwn = kMaxPairs / kThreads, kEach = kFewMaxExperts / kThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.tokens * a.topk;
     int e[kOwn], repeated = 0;
+    auto code = [&](int j) { return (uint16_t)((j * kThreads + tid) / a.topk << 5 | (j * kThreads + tid) % a.topk); };
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) {
         const int p = j * kThreads + tid;
@@ -210,7 +211,7 @@ __device__ __forceinline__ void make_plan(const FewTokensArgs& a, Plan& s, int* 
     cut = __syncthreads_or(cut);
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
-        if (e[j] >= 0) s.pair[atomicAdd(start + e[j], 1)] = (uint16_t)(j * kThreads + tid);
+        if (e[j] >= 0) s.pair[atomicAdd(start + e[j], 1)] = code(j);
     __syncthreads();
     if (!cut) return;
     int to[kOwn];
@@ -219,12 +220,12 @@ __device__ __forceinline__ void make_plan(const FewTokensArgs& a, Plan& s, int* 
         if (e[j] < 0) continue;
         const int begin = e[j] > 0 ? start[e[j] - 1] : 0, stop = start[e[j]];  // (each has moved on to the end of its own)
         to[j] = begin;
-        for (int i = begin; i < stop; ++i) to[j] += s.pair[i] < j * kThreads + tid;
+        for (int i = begin; i < stop; ++i) to[j] += s.pair[i] < code(j);
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
-        if (e[j] >= 0) s.pair[to[j]] = (uint16_t)(j * kThreads + tid);
+        if (e[j] >= 0) s.pair[to[j]] = code(j);
     __syncthreads();
 }
 
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
     for (; now.u < units; advance(now)) {
         const int block = now.block, at = s.group_start[now.group], n = (now.group + 1 < groups ? s.group_start[now.group + 1] : s.num_pairs) - at;
         const int mine = g < n ? s.pair[at + g] : -1;  // this lane's column
-        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (mine / a.topk) * a.x_stride;
+        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (mine >> 5) * a.x_stride;
         const int blocks_k = a.hidden / 128;
         const float* scales = kFp8 ? a.s13 + ((long long)s.group_expert[now.group] * (2 * a.inter / 128) + block * 16 / 128) * blocks_k : nullptr;
         float acc[2][4] = {};
@@ -422,10 +423,10 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
                 gate += reinterpret_cast<const float*>(red[team * kTeamWarps + w][0])[from];
                 up += reinterpret_cast<const float*>(red[team * kTeamWarps + w][1])[from];
             }
-            const int q = s.pair[at + c];
+            const int code = s.pair[at + c], q = (code >> 5) * a.topk + (code & 31);
             float weight = a.weights[q];
             if (s.repeated)
-                for (int k = q % a.topk + 1, z = q + 1; k < a.topk; ++k, ++z)
+                for (int z = q + 1; z < ((code >> 5) + 1) * a.topk; ++z)
                     if (a.idx[z] == a.idx[q]) weight += a.weights[z];
             const float v = silu(gate) * up * weight;
             const long long to = (long long)q * a.inter + i;
@@ -465,15 +466,15 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
     make_plan(a, s, reinterpret_cast<int*>(sums));
     const int groups = s.num_groups;
     const long long all = (long long)groups * boxes;
-    const int end = (int)(all * (rank + 1) / p.cluster), first = (int)(all * rank / p.cluster) + warp;  // this warp's boxes: every eighth from `first`, the groups' one after the other
+    // this warp's boxes: an equal share of the groups' boxes, laid out one after the other
+    const int share = rank * kWarps + warp, shares = p.cluster * kWarps, first = (int)(all * share / shares), end = (int)(all * (share + 1) / shares);
     struct Place {
         int b, group, j;
     };
     auto advance = [&](Place& at) {
-        at.b += kWarps;
-        at.j += kWarps;
-        while (at.j >= boxes) {
-            at.j -= boxes;
+        ++at.b;
+        if (++at.j == boxes) {
+            at.j = 0;
             ++at.group;
         }
     };
@@ -502,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (2 * t + i >= n) continue;
-            const int token = s.pair[at + 2 * t + i] / a.topk;
+            const int token = s.pair[at + 2 * t + i] >> 5;
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
             group = now.group;
             at = s.group_start[group];
             n = (group + 1 < groups ? s.group_start[group + 1] : s.num_pairs) - at;
-            mine = g < n ? s.pair[at + g] : -1;
+            mine = g < n ? (s.pair[at + g] >> 5) * a.topk + (s.pair[at + g] & 31) : -1;
             if constexpr (kFp8) scales = a.s2 + ((long long)s.group_expert[group] * (a.hidden / 128) + tile * kBoxRows / 128) * (a.inter / 128);
         }
         int4 w[2][2][2];
