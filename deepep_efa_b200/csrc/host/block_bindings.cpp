@@ -167,6 +167,56 @@ torch::Tensor select_experts_bwd(const torch::Tensor& logits_in, const torch::Te
     return dlogits;
 }
 
+// The two with gradients as nodes of the autograd graph. In C++, since a step's launches are short: choice and gradient of 8192 x 64, us, as a Python function 70, so XXX.
+struct RMSNorm : torch::autograd::Function<RMSNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
+                                                  const c10::optional<torch::Tensor>& residual, double eps) {
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = residual.has_value();
+        const auto [y, q, scales, total] = rms_norm(x, weight, residual, eps, true, false, false);
+        ctx->save_for_backward({residual.has_value() ? *total : x, weight});
+        if (residual.has_value()) return {*y, *total};
+        return {*y};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const bool residual = ctx->saved_data["residual"].toBool();
+        torch::Tensor dx, dw;
+        c10::optional<torch::Tensor> past;
+        if (residual && grads[1].defined()) past = grads[1];
+        if (grads[0].defined())
+            std::tie(dx, dw) = rms_norm_bwd(saved[0], saved[1], grads[0], past, ctx->saved_data["eps"].toDouble());
+        else if (past.has_value())
+            dx = *past;
+        return {dx, dw, residual ? dx : torch::Tensor(), torch::Tensor()};
+    }
+};
+torch::autograd::variable_list rms_norm_grad(const torch::Tensor& x, const torch::Tensor& weight, const c10::optional<torch::Tensor>& residual, double eps) {
+    return RMSNorm::apply(x, weight, residual, eps);
+}
+
+struct SelectExperts : torch::autograd::Function<SelectExperts> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& logits, int64_t topk, bool renormalize) {
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["renormalize"] = renormalize;
+        const auto [idx, weights] = select_experts(logits, topk, renormalize);
+        ctx->mark_non_differentiable({idx});
+        ctx->save_for_backward({logits, idx, weights});
+        return {idx, weights};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        torch::Tensor dlogits;
+        if (grads[1].defined()) dlogits = select_experts_bwd(saved[0], saved[1], saved[2], grads[1], ctx->saved_data["renormalize"].toBool());
+        return {dlogits, torch::Tensor(), torch::Tensor()};
+    }
+};
+std::tuple<torch::Tensor, torch::Tensor> select_experts_grad(const torch::Tensor& logits, int64_t topk, bool renormalize) {
+    const auto out = SelectExperts::apply(logits, topk, renormalize);
+    return {out[0], out[1]};
+}
+
 torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in, const torch::Tensor& weights_in, const torch::Tensor& w13, const torch::Tensor& w2,
                          c10::optional<torch::Tensor> s13, c10::optional<torch::Tensor> s2, int64_t first, c10::optional<torch::Tensor> out) {
     const char* what = "few_token_experts";
@@ -228,8 +278,10 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
 
 void bind_block(py::module_& m) {
     m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_grad", &rms_norm_grad);
     m.def("rms_norm_bwd", &rms_norm_bwd);
     m.def("select_experts", &select_experts);
+    m.def("select_experts_grad", &select_experts_grad);
     m.def("select_experts_bwd", &select_experts_bwd);
     m.def("few_tokens", &few_tokens);
 }

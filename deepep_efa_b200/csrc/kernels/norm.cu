@@ -119,104 +119,174 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
     }
 }
 
-// A CTA takes every gridDim.x-th row and keeps its share of the weight's gradient in registers.
-template <int C, bool kWide>
-__global__ void __launch_bounds__(1024) rms_norm_bwd_kernel(const NormBwdArgs a) {
+// Pairs of fp32 numbers in one register pair: sm_100 adds and multiplies them in one instruction.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair_of(float lo, float hi) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 of_pair(f32x2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void unpack8(const int4& v, f32x2 (&f)[4]) {
+    const uint32_t w[4] = {(uint32_t)v.x, (uint32_t)v.y, (uint32_t)v.z, (uint32_t)v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = pair_of(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
+template <bool kWide>
+__device__ __forceinline__ void load_weight8(const void* w, int chunk, f32x2 (&f)[4]) {
+    float g[8];
+    load_weight8<kWide>(w, chunk, g);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = pair_of(g[2 * j], g[2 * j + 1]);
+}
+__device__ __forceinline__ void copy16(uint32_t to, const int4* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+// A CTA takes every gridDim.x-th row and keeps its share of the weight's gradient in registers, and the weight, where rows are not too wide. A thread copies its own
+// chunks of the rows ahead into shared memory and reads them back alone, so that loads stay in flight over a row's sums without a barrier. Chunks past the
+// row's end, and a dtotal that is not there, are zeros in shared memory from the start. 8192 x 4096, us: row after row
+// straight to registers 62; rows ahead, 16 channels per thread 64; 32 per thread 60; math in pairs, weight kept 43 (its 268 MB at the measured copy rate: 41).
+template <int C, int S, int kMostThreads, bool kWide>
+__global__ void __launch_bounds__(kMostThreads) rms_norm_bwd_kernel(const NormBwdArgs a) {
+    extern __shared__ __align__(16) uint8_t ahead[];  // [S][three arrays][C * threads chunks of 16 bytes]
     __shared__ float2 s_sum[2][32];
+    constexpr bool kKeep = kMostThreads == 256;
+    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, n16 = a.hidden / 8, pitch = C * threads;
+    int4* own = reinterpret_cast<int4*>(ahead) + tid;
+    const uint32_t own_at = (uint32_t)__cvta_generic_to_shared(own);
+    for (int i = 0; i < S * 3 * C; ++i) own[i * threads] = make_int4(0, 0, 0, 0);
+    f32x2 dw[C][4], kept[kKeep ? C : 1][4];
     pdl_wait_predecessor();
     pdl_release_successor();
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, n16 = a.hidden / 8;
-    float dw[C][8];
 #pragma unroll
-    for (int c = 0; c < C; ++c)
+    for (int c = 0; c < C; ++c) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dw[c][j] = 0.f;
-    int parity = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
-        const int4* t = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.total) + row * a.total_stride);
-        const int4* d = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.dy) + row * a.dy_stride);
-        int4 tv[C], dv[C], uv[C];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
+        for (int j = 0; j < 4; ++j) dw[c][j] = 0;
+        if constexpr (kKeep) {
             const int i = c * threads + tid;
-            tv[c] = i < n16 ? ld_once(t + i) : make_int4(0, 0, 0, 0);
-            dv[c] = i < n16 ? ld_once(d + i) : make_int4(0, 0, 0, 0);
+            load_weight8<kWide>(a.weight, i < n16 ? i : 0, kept[c]);
         }
+    }
+    auto weight_of = [&](int c, f32x2 (&w)[4]) {
+        if constexpr (kKeep) {
 #pragma unroll
-        for (int c = 0; c < C; ++c) uv[c] = make_int4(0, 0, 0, 0);
-        if (a.dtotal != nullptr) {
-            const int4* u = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.dtotal) + row * a.dtotal_stride);
+            for (int j = 0; j < 4; ++j) w[j] = kept[c][j];
+        } else {
+            const int i = c * threads + tid;
+            load_weight8<kWide>(a.weight, i < n16 ? i : 0, w);
+        }
+    };
+    auto fetch = [&](long long row, int stage) {
+        if (row < a.rows) {
+            const int4* t = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.total) + row * a.total_stride) + tid;
+            const int4* d = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.dy) + row * a.dy_stride) + tid;
+            const int4* u = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.dtotal) + row * a.dtotal_stride) + tid;
+            const uint32_t to = own_at + stage * 3 * pitch * 16;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
-                const int i = c * threads + tid;
-                if (i < n16) uv[c] = ld_once(u + i);
+                if (c * threads + tid >= n16) continue;
+                copy16(to + c * threads * 16, t + c * threads);
+                copy16(to + (pitch + c * threads) * 16, d + c * threads);
+                if (a.dtotal != nullptr) copy16(to + (2 * pitch + c * threads) * 16, u + c * threads);
             }
         }
-        float squares = 0.f, inner = 0.f;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const float per_channel = 1.f / (float)a.hidden;
+    int parity = 0, stage = 0;
+#pragma unroll
+    for (int i = 0; i < S; ++i) fetch(blockIdx.x + (long long)i * gridDim.x, i);
+    for (long long row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S - 1) : "memory");
+        const int4* now = own + stage * 3 * pitch;
+        f32x2 squares2 = 0, inner2 = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int i = c * threads + tid;
-            float f[8], g[8], w[8];
-            unpack8(tv[c], f);
-            unpack8(dv[c], g);
-            load_weight8<kWide>(a.weight, i < n16 ? i : 0, w);
+            f32x2 f[4], g[4], w[4];
+            unpack8(now[c * threads], f);
+            unpack8(now[pitch + c * threads], g);
+            weight_of(c, w);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                squares = fmaf(f[j], f[j], squares);
-                inner = fmaf(g[j] * w[j], f[j], inner);
+            for (int j = 0; j < 4; ++j) {
+                squares2 = fma2(f[j], f[j], squares2);
+                inner2 = fma2(mul2(g[j], w[j]), f[j], inner2);
             }
         }
-        squares = warp_add(squares);
-        inner = warp_add(inner);
+        float squares = warp_add(of_pair(squares2).x + of_pair(squares2).y), inner = warp_add(of_pair(inner2).x + of_pair(inner2).y);
         if (lane == 0) s_sum[parity][tid >> 5] = make_float2(squares, inner);
         __syncthreads();  // (two buffers: a warp that is a row ahead writes the other one)
-        const float2 all = lane < threads / 32 ? s_sum[parity][lane] : make_float2(0.f, 0.f);
-        squares = warp_add(all.x);
-        inner = warp_add(all.y);
-        const float r = rsqrtf(squares / (float)a.hidden + a.eps), back = r * r * (inner / (float)a.hidden);
-        int4* o = reinterpret_cast<int4*>(a.dx) + row * n16;
+        squares = inner = 0.f;
+        for (int w = 0; w < threads / 32; ++w) {
+            const float2 part = s_sum[parity][w];
+            squares += part.x;
+            inner += part.y;
+        }
+        const float r = rsqrtf(fmaf(squares, per_channel, a.eps)), back = -r * r * r * (inner * per_channel);
+        const f32x2 r2 = pair_of(r, r), back2 = pair_of(back, back);
+        int4* o = reinterpret_cast<int4*>(a.dx) + row * n16 + tid;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const int i = c * threads + tid;
-            float f[8], g[8], w[8], u[8];
-            unpack8(tv[c], f);
-            unpack8(dv[c], g);
-            unpack8(uv[c], u);
-            load_weight8<kWide>(a.weight, i < n16 ? i : 0, w);
+            f32x2 f[4], g[4], w[4], u[4];
+            unpack8(now[c * threads], f);
+            unpack8(now[pitch + c * threads], g);
+            unpack8(now[2 * pitch + c * threads], u);
+            weight_of(c, w);
+            uint32_t out[4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                dw[c][j] = fmaf(g[j], f[j] * r, dw[c][j]);
-                u[j] = fmaf(r, fmaf(-back, f[j], g[j] * w[j]), u[j]);
+            for (int j = 0; j < 4; ++j) {
+                const f32x2 gr = mul2(g[j], r2);
+                dw[c][j] = fma2(gr, f[j], dw[c][j]);
+                const float2 v = of_pair(fma2(gr, w[j], fma2(back2, f[j], u[j])));
+                out[j] = f2_to_bf16x2(v.x, v.y);
             }
-            if (i < n16) o[i] = pack8(u);
+            if (c * threads + tid < n16) st_once(o + c * threads, make_int4((int)out[0], (int)out[1], (int)out[2], (int)out[3]));
         }
+        fetch(row + (long long)S * gridDim.x, stage);
+        stage = stage + 1 == S ? 0 : stage + 1;
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int i = c * threads + tid;
         if (i >= n16) continue;
         float4* p = reinterpret_cast<float4*>(a.partial + (size_t)blockIdx.x * a.hidden) + 2 * i;
-        p[0] = make_float4(dw[c][0], dw[c][1], dw[c][2], dw[c][3]);
-        p[1] = make_float4(dw[c][4], dw[c][5], dw[c][6], dw[c][7]);
+        p[0] = make_float4(of_pair(dw[c][0]).x, of_pair(dw[c][0]).y, of_pair(dw[c][1]).x, of_pair(dw[c][1]).y);
+        p[1] = make_float4(of_pair(dw[c][2]).x, of_pair(dw[c][2]).y, of_pair(dw[c][3]).x, of_pair(dw[c][3]).y);
     }
 }
 
 // dweight[i] = sum of the CTAs' partial sums, 32 channels per CTA, in a fixed order
 template <bool kWide>
-__global__ void __launch_bounds__(512) norm_dweight_kernel(const float* __restrict__ partial, void* __restrict__ dweight, int ctas, int hidden) {
-    __shared__ float s[16][33];
+__global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* __restrict__ partial, void* __restrict__ dweight, int ctas, int hidden) {
+    __shared__ float s[32][33];
     pdl_wait_predecessor();
     pdl_release_successor();
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
     float sum = 0.f;
-    if (i < hidden)
-        for (int c = w; c < ctas; c += 16) sum += partial[(size_t)c * hidden + i];
+    if (i < hidden) {
+#pragma unroll 8
+        for (int c = w; c < ctas; c += 32) sum += partial[(size_t)c * hidden + i];
+    }
     s[w][lane] = sum;
     __syncthreads();
     if (w != 0 || i >= hidden) return;
     sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) sum += s[j][lane];
+    for (int j = 0; j < 32; ++j) sum += s[j][lane];
     if constexpr (kWide)
         reinterpret_cast<float*>(dweight)[i] = sum;
     else
@@ -240,11 +310,37 @@ cudaError_t norm_forward(const NormArgs& a, int threads, cudaStream_t stream) {
     const dim3 grid((unsigned)a.rows);
     return a.weight_f32 ? launch_dependent(rms_norm_kernel<C, true>, grid, threads, 0, stream, a) : launch_dependent(rms_norm_kernel<C, false>, grid, threads, 0, stream, a);
 }
-template <int C>
-cudaError_t norm_backward(const NormBwdArgs& a, int threads, int ctas, cudaStream_t stream) {
-    const dim3 grid((unsigned)ctas);
-    return a.weight_f32 ? launch_dependent(rms_norm_bwd_kernel<C, true>, grid, threads, 0, stream, a)
-                        : launch_dependent(rms_norm_bwd_kernel<C, false>, grid, threads, 0, stream, a);
+
+// The backward pass: rows that a CTA fetches ahead, and CTAs per SM.
+struct BwdShape {
+    Shape row;
+    int stages, per_sm;
+    size_t smem;
+};
+BwdShape bwd_shape_of(int hidden) {
+    // Many channels per thread: what a row costs a warp beside its channels (two sums over the CTA, addresses) was two thirds of the instructions with 16 of them.
+    const int n16 = (hidden + 7) / 8, chunks = n16 >= 512 ? 4 : n16 >= 256 ? 2 : 1;
+    BwdShape b;
+    b.row = {chunks, ((n16 + chunks - 1) / chunks + 31) / 32 * 32};
+    const size_t bytes = (size_t)3 * chunks * b.row.threads * 16, most = 220 * 1024;
+    b.stages = 12 * bytes <= most ? 3 : 2 * bytes <= most ? 2 : 1;
+    b.smem = b.stages * bytes;
+    const int by_smem = (int)(most / (b.smem + 2048)), by_threads = (chunks == 4 ? 512 : 1024) / b.row.threads;
+    b.per_sm = by_smem < by_threads ? by_smem : by_threads;
+    if (b.per_sm < 1) b.per_sm = 1;
+    return b;
+}
+template <int C, int S, int kMostThreads, bool kWide>
+cudaError_t norm_backward_as(const NormBwdArgs& a, const BwdShape& b, int ctas, cudaStream_t stream) {
+    const cudaError_t e = cudaFuncSetAttribute(rms_norm_bwd_kernel<C, S, kMostThreads, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)b.smem);
+    return e != cudaSuccess ? e : launch_dependent(rms_norm_bwd_kernel<C, S, kMostThreads, kWide>, dim3((unsigned)ctas), b.row.threads, b.smem, stream, a);
+}
+template <bool kWide>
+cudaError_t norm_backward(const NormBwdArgs& a, const BwdShape& b, int ctas, cudaStream_t stream) {
+    if (b.row.chunks == 1) return norm_backward_as<1, 3, 256, kWide>(a, b, ctas, stream);
+    if (b.row.chunks == 2) return norm_backward_as<2, 3, 256, kWide>(a, b, ctas, stream);
+    if (b.row.threads <= 256) return b.stages == 3 ? norm_backward_as<4, 3, 256, kWide>(a, b, ctas, stream) : norm_backward_as<4, 2, 256, kWide>(a, b, ctas, stream);
+    return b.stages == 2 ? norm_backward_as<4, 2, 1024, kWide>(a, b, ctas, stream) : norm_backward_as<4, 1, 1024, kWide>(a, b, ctas, stream);
 }
 
 }  // namespace
@@ -257,8 +353,7 @@ cudaError_t launch_rms_norm(const NormArgs& a, cudaStream_t stream) {
 }
 
 int norm_bwd_ctas(long long rows, int hidden, int num_sms) {
-    const Shape s = shape_of(num_sms + 1ll, hidden, num_sms);
-    const long long most = (long long)num_sms * (s.threads >= 1024 ? 1 : 1024 / s.threads);
+    const long long most = (long long)num_sms * bwd_shape_of(hidden).per_sm;
     return (int)(rows < most ? rows : most);
 }
 
@@ -266,15 +361,13 @@ cudaError_t launch_rms_norm_bwd(const NormBwdArgs& a, int num_sms, cudaStream_t 
     if (a.hidden <= 0 || (a.hidden & 7) != 0 || a.hidden > kNormMaxHidden) return cudaErrorInvalidValue;
     const int ctas = norm_bwd_ctas(a.rows, a.hidden, num_sms);
     if (ctas > 0) {
-        const Shape s = shape_of(num_sms + 1ll, a.hidden, num_sms);
-        const cudaError_t e = s.chunks == 1   ? norm_backward<1>(a, s.threads, ctas, stream)
-                              : s.chunks == 2 ? norm_backward<2>(a, s.threads, ctas, stream)
-                                              : norm_backward<4>(a, s.threads, ctas, stream);
+        const BwdShape b = bwd_shape_of(a.hidden);
+        const cudaError_t e = a.weight_f32 ? norm_backward<true>(a, b, ctas, stream) : norm_backward<false>(a, b, ctas, stream);
         if (e != cudaSuccess) return e;
     }
     const dim3 grid((unsigned)((a.hidden + 31) / 32));
-    return a.weight_f32 ? launch_dependent(norm_dweight_kernel<true>, grid, 512, 0, stream, (const float*)a.partial, a.dweight, ctas, a.hidden)
-                        : launch_dependent(norm_dweight_kernel<false>, grid, 512, 0, stream, (const float*)a.partial, a.dweight, ctas, a.hidden);
+    return a.weight_f32 ? launch_dependent(norm_dweight_kernel<true>, grid, 1024, 0, stream, (const float*)a.partial, a.dweight, ctas, a.hidden)
+                        : launch_dependent(norm_dweight_kernel<false>, grid, 1024, 0, stream, (const float*)a.partial, a.dweight, ctas, a.hidden);
 }
 
 }  // namespace dx

@@ -28,22 +28,17 @@ def _check_cpu(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.T
         raise ValueError("deepep_efa_b200.rms_norm: residual must be of x's shape and type")
 
 
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.dim() == 2 else t.reshape(-1, t.size(-1))
-
-
 class _RMSNorm(torch.autograd.Function):
+    """The CPU form."""
+
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
         ctx.eps, ctx.has_residual = eps, residual is not None
         ctx.set_materialize_grads(False)
-        if x.is_cuda:
-            y, _, _, total = _ext.load().rms_norm(x, weight, residual, eps, True, False, False)
-        else:
-            _check_cpu(x, weight, residual)
-            total = None if residual is None else _total(x, residual)
-            t = (x if residual is None else total).float()
-            y = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()).to(x.dtype)
+        _check_cpu(x, weight, residual)
+        total = None if residual is None else _total(x, residual)
+        t = (x if residual is None else total).float()
+        y = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()).to(x.dtype)
         ctx.save_for_backward(x if residual is None else total, weight)
         return y if residual is None else (y, total)
 
@@ -52,8 +47,6 @@ class _RMSNorm(torch.autograd.Function):
         total, weight = ctx.saved_tensors
         if dy is None:
             dx, dw = dtotal, None
-        elif total.is_cuda:
-            dx, dw = _ext.load().rms_norm_bwd(total, weight, dy, dtotal, ctx.eps)
         else:
             t, g = total.float(), dy.float()
             r = torch.rsqrt(t.square().mean(-1, keepdim=True) + ctx.eps)
@@ -68,10 +61,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     """The norm of the rows of ``x`` (bf16 ``[..., H]``, ``H`` a multiple of 8 up to 32768; ``weight`` bf16 or fp32 ``[H]``). Returns ``y``, or with a ``residual``
     of ``x``'s shape ``(y, x + residual)``. Differentiable in all three; ``weight``'s gradient is summed in fp32 in a fixed order and has its type."""
     shape = x.shape
-    if x.dim() == 2:
-        return _RMSNorm.apply(x, weight, residual, eps)
-    out = _RMSNorm.apply(_rows(x), weight, _rows(residual), eps)
-    return out.view(shape) if residual is None else (out[0].view(shape), out[1].view(shape))
+    if x.dim() != 2:
+        x, residual = x.reshape(-1, shape[-1]), None if residual is None else residual.reshape(-1, shape[-1])
+    if x.is_cuda:
+        out = _ext.load().rms_norm_grad(x, weight, residual, eps)
+    else:
+        out = _RMSNorm.apply(x, weight, residual, eps)
+        out = (out,) if residual is None else out
+    if len(shape) != 2:
+        out = [o.view(shape) for o in out]
+    return out[0] if residual is None else (out[0], out[1])
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *, eps: float = 1e-6, round_scale: bool = False,

@@ -12,22 +12,21 @@ from .. import _ext
 
 
 class _SelectExperts(torch.autograd.Function):
+    """The CPU form."""
+
     @staticmethod
     def forward(ctx, logits, num_topk, renormalize):
         ctx.renormalize = renormalize
         ctx.set_materialize_grads(False)
-        if logits.is_cuda:
-            idx, weights = _ext.load().select_experts(logits, num_topk, renormalize)
-        else:
-            if logits.dim() != 2 or not 1 <= num_topk <= min(32, logits.size(1)) or logits.size(1) > 1024:
-                raise ValueError("deepep_efa_b200.select_experts: logits must be [T, E], num_topk 1 to 32 and at most E, E at most 1024")
-            values, order = torch.sort(logits.float(), dim=-1, descending=True, stable=True)
-            values, order = values[:, :num_topk], order[:, :num_topk]
-            gone = values == -torch.inf
-            idx = order.masked_fill(gone, -1)
-            top = values[:, :1].masked_fill(gone[:, :1], 0.0)
-            total = torch.exp((values if renormalize else logits.float()) - top).sum(-1, keepdim=True)
-            weights = torch.where(gone, torch.zeros_like(values), torch.exp(values - top) / total)
+        if logits.dim() != 2 or not 1 <= num_topk <= min(32, logits.size(1)) or logits.size(1) > 1024:
+            raise ValueError("deepep_efa_b200.select_experts: logits must be [T, E], num_topk 1 to 32 and at most E, E at most 1024")
+        values, order = torch.sort(logits.float(), dim=-1, descending=True, stable=True)
+        values, order = values[:, :num_topk], order[:, :num_topk]
+        gone = values == -torch.inf
+        idx = order.masked_fill(gone, -1)
+        top = values[:, :1].masked_fill(gone[:, :1], 0.0)
+        total = torch.exp((values if renormalize else logits.float()) - top).sum(-1, keepdim=True)
+        weights = torch.where(gone, torch.zeros_like(values), torch.exp(values - top) / total)
         ctx.mark_non_differentiable(idx)
         ctx.save_for_backward(logits, idx, weights)
         return idx, weights
@@ -37,8 +36,6 @@ class _SelectExperts(torch.autograd.Function):
         if dweights is None:
             return None, None, None
         logits, idx, weights = ctx.saved_tensors
-        if logits.is_cuda:
-            return _ext.load().select_experts_bwd(logits, idx, weights, dweights, ctx.renormalize), None, None
         chosen = idx >= 0
         inner = torch.where(chosen, weights * dweights, torch.zeros_like(weights)).sum(-1, keepdim=True)
         dlogits = torch.zeros(logits.shape, dtype=torch.float32) if ctx.renormalize else -inner * torch.softmax(logits.float(), -1).nan_to_num()
@@ -52,4 +49,8 @@ def select_experts(logits: torch.Tensor, num_topk: int, *, renormalize: bool = T
     A token gets its ``num_topk`` largest logits in falling order, of equal ones the lowest index first, NaN before all others. Weights are the softmax over the
     chosen logits, or with ``renormalize=False`` their probabilities among all experts. An expert whose logit is ``-inf`` is not chosen: what then is left over of
     a row is ``-1`` with weight 0 (dispatch skips it). Differentiable in ``logits``."""
-    return _SelectExperts.apply(logits, num_topk, renormalize)
+    if not logits.is_cuda:
+        return _SelectExperts.apply(logits, num_topk, renormalize)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _ext.load().select_experts_grad(logits, num_topk, renormalize)
+    return _ext.load().select_experts(logits, num_topk, renormalize)
