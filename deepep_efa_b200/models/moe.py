@@ -15,6 +15,10 @@ Two execution paths share the structure:
   and starts on an expert as soon as that expert's arrival counter reaches the expected total; the second grouped
   GEMM's epilogue stores every output row straight into the stage of the token's home rank over NVLink, so the
   combine that remains is a cross-rank flag exchange and a local weighted sum.
+* **a few tokens**: ``forward_few_tokens`` is a decode step of up to 32 tokens on a rank that has all experts: no dispatch and no combine, two
+  kernels that read the chosen experts' weights once.
+
+``MoEBlock`` puts a layer into a residual stream: addition, root-mean-square norm, choice of the experts, experts.
 
 The reference is a communication library only and has no model code; this module is the model-side user of the
 API that the benchmark configurations (fused MoE forward, MoE training step) call for.
@@ -22,14 +26,17 @@ API that the benchmark configurations (fused MoE forward, MoE training step) cal
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
 from ..ops import grouped_gemm as gg
+from ..ops.few_tokens import few_token_experts
+from ..ops.norm import rms_norm, rms_norm_fp8
 from ..ops.permute import build_expert_plan, permute, unpermute_weighted
+from ..ops.router import select_experts
 
 EXPERT_ALIGNMENT = 128
 
@@ -145,6 +152,10 @@ class MoELayer(nn.Module):
         topk_logits, topk_idx = logits.topk(self.cfg.num_topk, dim=-1)
         return topk_idx.to(torch.int64), torch.softmax(topk_logits.float(), dim=-1)
 
+    def choose(self, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The same choice as :meth:`route` by one kernel (:func:`select_experts`), and by a second one backwards; of equal logits the lowest expert comes first."""
+        return select_experts(x.to(self.gate.dtype) @ self.gate.t(), self.cfg.num_topk)
+
     # -- BF16 path with autograd ----------------------------------------------------------------------------
     def forward(self, x: torch.Tensor, topk_idx: Optional[torch.Tensor] = None, topk_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
         if topk_idx is None:
@@ -200,25 +211,33 @@ class MoELayer(nn.Module):
                         gg.build_sf_atoms_b(s2, n2, wide=True) if n2 % 256 == 0 else gg.build_sf_atoms_b(s2, n2, wide=False))
 
     @torch.no_grad()
-    def forward_fp8(self, x: torch.Tensor, topk_idx: Optional[torch.Tensor] = None, topk_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Forward only: FP8 on the wire and in both expert GEMMs, SwiGLU fused into the first GEMM, BF16 combine."""
+    def forward_fp8(self, x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_idx: Optional[torch.Tensor] = None,
+                    topk_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Forward only: FP8 on the wire and in both expert GEMMs, SwiGLU fused into the first GEMM, BF16 combine.
+
+        ``x`` may come quantised, as ``(e4m3 rows, fp32 scales per 128 channels)`` with its ids and weights (``rms_norm_fp8``; scales are powers of two
+        where ``prepare_fp8`` chose native block scaling)."""
         from .. import _ext
         C = _ext.load()
         if self._fp8 is None:
             self.prepare_fp8()
         (w13, s13), (w2, s2) = self._fp8
+        quantised = isinstance(x, tuple)
         if topk_idx is None:
+            if quantised:
+                raise ValueError("deepep_efa_b200.forward_fp8: quantised rows come with their expert ids and weights")
             topk_idx, topk_weights = self.route(x)
+        num_tokens = x[0].size(0) if quantised else x.size(0)
         buf = self.buffer
         mx = getattr(self, "_mx", None)
         per_rank, _, per_expert, in_rank, _ = buf.get_dispatch_layout(topk_idx, self.cfg.num_experts)
         (rx, rs), recv_idx, recv_w, counts, handle, _ = buf.dispatch(
             x, num_tokens_per_rank=per_rank, is_token_in_rank=in_rank, num_tokens_per_expert=per_expert, topk_idx=topk_idx,
-            topk_weights=topk_weights, expert_alignment=EXPERT_ALIGNMENT, quantize_fp8=True, round_scale=mx is not None)
+            topk_weights=topk_weights, expert_alignment=EXPERT_ALIGNMENT, quantize_fp8=not quantised, round_scale=mx is not None and not quantised)
         plan = build_expert_plan(recv_idx, counts)
         if mx is not None:
             # padding rows of the plan carry all-zero data; whatever exponent their zero scale maps to does not matter
-            columns = _token_columns(buf.group_size * x.size(0) * self.cfg.num_topk / self.cfg.num_experts, w13.numel() + w2.numel(), self.cfg.hidden)
+            columns = _token_columns(buf.group_size * num_tokens * self.cfg.num_topk / self.cfg.num_experts, w13.numel() + w2.numel(), self.cfg.hidden)
             if columns or plan.num_rows >= WIDE_TILE_MIN_ROWS_PER_EXPERT * self.num_local_experts:
                 # the first GEMM quantises its own output: a wide tile holds one whole scale block of a row
                 y_perm = C.fp8_experts(rx, rs, plan.src_row, w13, w2, plan.m_offsets, plan.m_ends, mx[0], mx[3], GEMM_TIMEOUT_MS, columns)
@@ -311,6 +330,52 @@ class MoELayer(nn.Module):
                            early_table=True, rows_hint=arriving)
         out, _, _ = buf.low_latency_combine(y, topk_idx, topk_weights, handle, zero_copy=True)
         return out
+
+    # -- decode without an exchange -------------------------------------------------------------------------------
+    @torch.no_grad()
+    def forward_few_tokens(self, x: torch.Tensor, topk_idx: Optional[torch.Tensor] = None, topk_weights: Optional[torch.Tensor] = None, fp8: bool = True) -> torch.Tensor:
+        """Forward only, up to 32 tokens, on a rank that holds every expert: no dispatch, no combine, no host synchronisation (see
+        :func:`few_token_experts`). ``fp8=True`` reads the e4m3 weights (``prepare_fp8``), ``False`` the bf16 parameters; activations keep 16 bits either way, so results are
+        nearer to the bf16 layer than those of the paths that send e4m3 rows."""
+        if self.buffer.group_size != 1:
+            raise ValueError("deepep_efa_b200.forward_few_tokens: this rank holds a part of the experts; use forward_low_latency")
+        if topk_idx is None:
+            topk_idx, topk_weights = self.choose(x)
+        if not fp8:
+            return few_token_experts(x, topk_idx, topk_weights, self.w13, self.w2)
+        if self._fp8 is None:
+            self.prepare_fp8()
+        (w13, s13), (w2, s2) = self._fp8
+        return few_token_experts(x, topk_idx, topk_weights, w13, w2, w13_scales=s13, w2_scales=s2)
+
+
+class MoEBlock(nn.Module):
+    """A layer of experts in a residual stream: ``total = x + residual``, ``y = experts(norm(total))``. Every form returns ``(y, total)``: the next block adds ``y`` to
+    ``total`` in its own norm, so the stream is read and written once per block."""
+
+    def __init__(self, cfg: MoEConfig, buffer, device: Optional[torch.device] = None, seed: int = 0, eps: float = 1e-6) -> None:
+        super().__init__()
+        self.moe, self.eps = MoELayer(cfg, buffer, device, seed), eps
+        self.norm = nn.Parameter(torch.ones(cfg.hidden, dtype=torch.float32, device=self.moe.gate.device))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """BF16, with gradients."""
+        y, total = (rms_norm(x, self.norm, eps=self.eps), x) if residual is None else rms_norm(x, self.norm, residual, self.eps)
+        return self.moe(y, *self.moe.choose(y)), total
+
+    @torch.no_grad()
+    def forward_fp8(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Prefill: the norm writes the rows that the dispatch sends (see :meth:`MoELayer.forward_fp8`)."""
+        if self.moe._fp8 is None:
+            self.moe.prepare_fp8()
+        rows, y, total = rms_norm_fp8(x, self.norm, residual, eps=self.eps, round_scale=getattr(self.moe, "_mx", None) is not None)
+        return self.moe.forward_fp8(rows, *self.moe.choose(y)), x if total is None else total
+
+    @torch.no_grad()
+    def forward_few_tokens(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, fp8: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Decode of up to 32 tokens on a rank that holds every expert (see :meth:`MoELayer.forward_few_tokens`); it can be captured into a graph."""
+        y, total = (rms_norm(x, self.norm, eps=self.eps), x) if residual is None else rms_norm(x, self.norm, residual, self.eps)
+        return self.moe.forward_few_tokens(y, *self.moe.choose(y), fp8=fp8), total
 
 
 # ---------------------------------------------------------------------------------------------------------
