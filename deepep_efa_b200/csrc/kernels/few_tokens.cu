@@ -25,6 +25,8 @@
 
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "block_api.h"
 #include "launch.cuh"
 #include "tc_prims.cuh"
@@ -40,7 +42,8 @@ constexpr int kBoxBytes = kBoxRows * 128;
 constexpr int kMostStages = 3;
 constexpr int kCols = 8;  // selections that are multiplied at a time
 constexpr int kMaxPairs = kFewMaxTokens * kFewMaxTopk;
-constexpr int kTeamWarps = 4;  // warps that share a unit of the first launch
+constexpr int kTeamWarps = 4;  // warps that share a unit of the first launch: its 16 x 8 hidden values are one for each of their threads
+static_assert(kTeamWarps * 32 == 16 * kCols, "");
 
 // What a CTA plans by: the selections in the order of their experts, and groups of up to eight of one expert.
 struct Plan {
@@ -148,7 +151,40 @@ __device__ __forceinline__ uint32_t scale_half2(uint32_t v, __half2 by) {
 // Lists the selections by expert and cuts each expert's into groups of up to eight. Every CTA does this for itself: at most 1024 ids. Where a token names an
 // expert twice, the first of the selections stands for both (the first launch adds up their weights). The selections of an expert that has one group come in any order
 // (a column's result does not depend on its place); those of one that has more are sorted, since all CTAs have to cut them alike.
+__device__ __forceinline__ void make_short_plan(const FewTokensArgs& a, Plan& s) {  // up to 32 selections: one warp, without shared memory in between
+    const int lane = lane_id(), pairs = a.tokens * a.topk;
+    const int64_t id = lane < pairs ? a.idx[lane] : -1, local = id - a.first;
+    const bool here = id >= 0 && local >= 0 && local < a.experts;
+    const int token = lane / a.topk;
+    const uint32_t before = (1u << lane) - 1, of_token = before & ~((1u << (token * a.topk & 31)) - 1);
+    uint32_t same = __match_any_sync(0xffffffffu, here ? (int)local : -1 - lane);
+    const bool again = here && (same & of_token) != 0;
+    same &= __ballot_sync(0xffffffffu, here && !again);
+    const int rank = __popc(same & before), n = __popc(same);
+    const bool first = here && !again && rank == 0;
+    const int mine = first ? n + (((n + kCols - 1) / kCols) << 16) : 0, incl = warp_incl_scan(mine), total = __shfl_sync(0xffffffffu, incl, 31);
+    const int start = __shfl_sync(0xffffffffu, (incl - mine) & 0xffff, same != 0 ? __ffs(same) - 1 : 0);
+    if (here && !again) s.pair[start + rank] = (uint16_t)(token << 5 | (lane - token * a.topk));
+    if (first) {
+        int g = (incl - mine) >> 16;
+        for (int c = 0; c < n; c += kCols, ++g) {
+            s.group_expert[g] = (uint16_t)local;
+            s.group_start[g] = (uint16_t)(start + c);
+        }
+    }
+    const uint32_t repeated = __ballot_sync(0xffffffffu, again);
+    if (lane == 0) {
+        s.num_pairs = total & 0xffff;
+        s.num_groups = total >> 16;
+        s.repeated = repeated != 0;
+    }
+}
 __device__ __forceinline__ void make_plan(const FewTokensArgs& a, Plan& s, int* start) {
+    if (a.tokens * a.topk <= 32) {
+        if (threadIdx.x < 32) make_short_plan(a, s);
+        __syncthreads();
+        return;
+    }
     constexpr int kOwn = kMaxPairs / kThreads, kEach = kFewMaxExperts / kThreads;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, pairs = a.tokens * a.topk;
     int e[kOwn], repeated = 0;
@@ -374,6 +410,9 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
         const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(a.x) + (mine >> 5) * a.x_stride;
         const int blocks_k = a.hidden / 128;
         const float* scales = kFp8 ? a.s13 + ((long long)s.group_expert[now.group] * (2 * a.inter / 128) + block * 16 / 128) * blocks_k : nullptr;
+        // this thread's hidden value: column `c`, row `r` of the unit
+        const int o = member * 32 + lane, r = o & 15, c = o >> 4, code = c < n ? s.pair[at + c] : 0, q = (code >> 5) * a.topk + (code & 31);
+        const float first_weight = c < n ? a.weights[q] : 0.f;
         float acc[2][4] = {};
         for (; j < boxes; j += kTeamWarps) {
             constexpr int kPieces = kFp8 ? 4 : 2;
@@ -415,16 +454,15 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
 #pragma unroll
         for (int m = 0; m < 2; ++m) red[warp][m][lane] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
         meet();
-        for (int o = member * 32 + lane; o < 16 * n; o += kTeamWarps * 32) {
-            const int r = o & 15, c = o >> 4, i = block * 16 + r, from = (lane_row_of(r & 7) * 4 + (c >> 1)) * 4 + ((r >> 3) << 1) + (c & 1);
+        if (c < n) {
+            const int i = block * 16 + r, from = (lane_row_of(r & 7) * 4 + (c >> 1)) * 4 + ((r >> 3) << 1) + (c & 1);
             float gate = 0.f, up = 0.f;
 #pragma unroll
             for (int w = 0; w < kTeamWarps; ++w) {
                 gate += reinterpret_cast<const float*>(red[team * kTeamWarps + w][0])[from];
                 up += reinterpret_cast<const float*>(red[team * kTeamWarps + w][1])[from];
             }
-            const int code = s.pair[at + c], q = (code >> 5) * a.topk + (code & 31);
-            float weight = a.weights[q];
+            float weight = first_weight;
             if (s.repeated)
                 for (int z = q + 1; z < ((code >> 5) + 1) * a.topk; ++z)
                     if (a.idx[z] == a.idx[q]) weight += a.weights[z];
@@ -630,7 +668,10 @@ cudaError_t launch_both(FewParams& p, int num_sms, cudaStream_t stream) {
     const size_t up_smem = smem_bytes(true, 1), down_smem = smem_bytes(false, a.tokens);
     cudaError_t e = cudaFuncSetAttribute(few_up_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)up_smem);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(few_down_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_smem);
-    if (e == cudaSuccess) e = launch_dependent(few_up_kernel<kFp8>, dim3((unsigned)(2 * num_sms)), kThreads, up_smem, stream, up, p);
+    // No more CTAs than there can be units for: beside fewer than two per SM the second launch finds room at once.
+    const long long units = (long long)std::min(a.tokens * a.topk, a.experts + a.tokens * a.topk / kCols) * ((a.inter + 15) / 16), teams = kWarps / kTeamWarps;
+    const int up_ctas = (int)std::min<long long>(2 * num_sms, (units + teams - 1) / teams);
+    if (e == cudaSuccess) e = launch_dependent(few_up_kernel<kFp8>, dim3((unsigned)up_ctas), kThreads, up_smem, stream, up, p);
     if (e != cudaSuccess) return e;
     // as many CTAs as two per SM hold
     const int tiles = (a.hidden + kBoxRows - 1) / kBoxRows;
