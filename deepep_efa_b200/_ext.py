@@ -128,7 +128,7 @@ def build(verbose: bool = False, force: bool = False):
 
 def load():
     """Return the native module, building it on first use."""
-    return build()
+    return _MODULE if _MODULE is not None else build()
 
 
 def is_built() -> bool:

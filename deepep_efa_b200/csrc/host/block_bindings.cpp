@@ -1,5 +1,6 @@
 // Python bindings of what stands around the routed experts of a block: norm, choice of the experts, experts for a few tokens.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
@@ -37,6 +38,15 @@ bool rows_fit(const torch::Tensor& t) {
 }
 torch::Tensor fitting(const torch::Tensor& t) { return rows_fit(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// Short steps wait for the host, which an allocation through the dispatcher takes a microsecond of.
+torch::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const torch::Tensor& like) { return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt); }
+
+// Refuses to drop a graph silently.
+void forward_only(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
+    if (!at::GradMode::is_enabled()) return;
+    for (const torch::Tensor* t : tensors) DXB_CHECK(!t->requires_grad(), what, "forward only; call it under torch.no_grad()");
+}
+
 int sms_of(const torch::Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
 
 // x [N, H] (+ residual) -> (y, q, scales, total), with None for what was not asked for
@@ -56,17 +66,16 @@ std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>, c10::opti
     const torch::Tensor x = fitting(x_in), res = residual.has_value() ? fitting(*residual) : x;
     const torch::Tensor w = weight.is_contiguous() && aligned16(weight) ? weight : weight.clone(at::MemoryFormat::Contiguous);
     c10::optional<torch::Tensor> y, q, scales, total;
-    const auto bf16 = x.options().requires_grad(false);
     dx::NormArgs a{};
-    if (rows) a.y = (y = torch::empty({N, H}, bf16))->data_ptr();
+    if (rows) a.y = (y = fresh({N, H}, at::kBFloat16, x))->data_ptr();
     if (quantize) {
-        a.q = static_cast<uint8_t*>((q = torch::empty({N, H}, bf16.dtype(torch::kFloat8_e4m3fn)))->data_ptr());
-        a.scales = (scales = torch::empty({N, H / 128}, bf16.dtype(torch::kFloat32)))->data_ptr<float>();
+        a.q = static_cast<uint8_t*>((q = fresh({N, H}, at::kFloat8_e4m3fn, x))->data_ptr());
+        a.scales = (scales = fresh({N, H / 128}, at::kFloat, x))->data_ptr<float>();
     }
     if (residual.has_value()) {
         a.residual = res.data_ptr();
         a.residual_stride = res.stride(0);
-        a.total = (total = torch::empty({N, H}, bf16))->data_ptr();
+        a.total = (total = fresh({N, H}, at::kBFloat16, x))->data_ptr();
     }
     a.x = x.data_ptr();
     a.x_stride = x.stride(0);
@@ -78,6 +87,14 @@ std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>, c10::opti
     a.eps = (float)eps;
     launched(dx::launch_rms_norm(a, stream_of(x)), what);
     return {y, q, scales, total};
+}
+
+// ((q, scales), y or None, total or None)
+std::tuple<std::tuple<torch::Tensor, torch::Tensor>, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> rms_norm_fp8(
+    const torch::Tensor& x, const torch::Tensor& weight, const c10::optional<torch::Tensor>& residual, double eps, bool round_scale, bool keep_rows) {
+    forward_only("rms_norm_fp8", {&x, &weight, residual.has_value() ? &*residual : &x});
+    const auto [y, q, scales, total] = rms_norm(x, weight, residual, eps, keep_rows, true, round_scale);
+    return {{*q, *scales}, y, total};
 }
 
 // -> (dx, dweight)
@@ -95,8 +112,7 @@ std::tuple<torch::Tensor, torch::Tensor> rms_norm_bwd(const torch::Tensor& total
     const torch::Tensor t = fitting(total_in), dy = fitting(dy_in), dt = dtotal.has_value() ? fitting(*dtotal) : dy;
     const torch::Tensor w = weight.is_contiguous() && aligned16(weight) ? weight : weight.clone(at::MemoryFormat::Contiguous);
     const int sms = sms_of(t), ctas = dx::norm_bwd_ctas(N, (int)H, sms);
-    const auto opt = t.options().requires_grad(false);
-    const torch::Tensor dx_out = torch::empty({N, H}, opt), dw = torch::empty({H}, opt.dtype(w.scalar_type())), partial = torch::empty({ctas, H}, opt.dtype(torch::kFloat32));
+    const torch::Tensor dx_out = fresh({N, H}, at::kBFloat16, t), dw = fresh({H}, w.scalar_type(), t), partial = fresh({ctas, H}, at::kFloat, t);
     dx::NormBwdArgs a{};
     a.total = t.data_ptr();
     a.dy = dy.data_ptr();
@@ -137,8 +153,7 @@ std::tuple<torch::Tensor, torch::Tensor> select_experts(const torch::Tensor& log
     dx::SelectArgs a = select_args(what, logits_in, topk, renormalize);
     c10::cuda::CUDAGuard guard(logits_in.device());
     const torch::Tensor logits = logit_rows(logits_in);
-    const auto opt = logits.options().requires_grad(false);
-    const torch::Tensor idx = torch::empty({a.tokens, a.topk}, opt.dtype(torch::kInt64)), weights = torch::empty({a.tokens, a.topk}, opt.dtype(torch::kFloat32));
+    const torch::Tensor idx = fresh({a.tokens, a.topk}, at::kLong, logits), weights = fresh({a.tokens, a.topk}, at::kFloat, logits);
     a.logits = logits.data_ptr();
     a.logits_stride = logits.stride(0);
     a.idx = idx.data_ptr<int64_t>();
@@ -156,7 +171,7 @@ torch::Tensor select_experts_bwd(const torch::Tensor& logits_in, const torch::Te
     DXB_CHECK(fits(weights) && weights.scalar_type() == torch::kFloat32 && weights.is_contiguous(), what, "weights must be contiguous fp32 [T, K] on the logits' device");
     DXB_CHECK(fits(dweights_in) && dweights_in.scalar_type() == torch::kFloat32, what, "the weights' gradient must be fp32 [T, K] on the logits' device");
     c10::cuda::CUDAGuard guard(logits_in.device());
-    const torch::Tensor logits = logit_rows(logits_in), dweights = dweights_in.contiguous(), dlogits = torch::empty({a.tokens, a.experts}, logits.options().requires_grad(false));
+    const torch::Tensor logits = logit_rows(logits_in), dweights = dweights_in.contiguous(), dlogits = fresh({a.tokens, a.experts}, logits.scalar_type(), logits);
     a.logits = logits.data_ptr();
     a.logits_stride = logits.stride(0);
     a.idx = idx.data_ptr<int64_t>();
@@ -167,7 +182,7 @@ torch::Tensor select_experts_bwd(const torch::Tensor& logits_in, const torch::Te
     return dlogits;
 }
 
-// The two with gradients as nodes of the autograd graph. In C++, since a step's launches are short: choice and gradient of 8192 x 64, us, as a Python function 70, so XXX.
+// The two with gradients as nodes of the autograd graph. In C++, since a step's launches are short: choice and gradient of 8192 x 64, us, as a Python function 70, so 58.
 struct RMSNorm : torch::autograd::Function<RMSNorm> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
                                                   const c10::optional<torch::Tensor>& residual, double eps) {
@@ -221,6 +236,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
                          c10::optional<torch::Tensor> s13, c10::optional<torch::Tensor> s2, int64_t first, c10::optional<torch::Tensor> out) {
     const char* what = "few_token_experts";
     const auto dev = x_in.device();
+    forward_only(what, {&x_in, &weights_in, &w13, &w2});
     DXB_CHECK(x_in.is_cuda() && x_in.dim() == 2 && x_in.scalar_type() == torch::kBFloat16, what, "x must be a CUDA bf16 matrix [T, H]");
     const int64_t T = x_in.size(0), H = x_in.size(1);
     DXB_CHECK(T <= dx::kFewMaxTokens, what, "at most 32 tokens");
@@ -248,7 +264,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
               "out must be contiguous bf16 [T, H] on x's device");
     c10::cuda::CUDAGuard guard(dev);
     const torch::Tensor x = fitting(x_in), idx = idx_in.contiguous(), weights = weights_in.contiguous();
-    const torch::Tensor y = out.has_value() ? *out : torch::empty({T, H}, x.options().requires_grad(false));
+    const torch::Tensor y = out.has_value() ? *out : fresh({T, H}, at::kBFloat16, x);
     dx::FewTokensArgs a{};
     a.x = x.data_ptr();
     a.x_stride = x.stride(0);
@@ -268,7 +284,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     a.fp8 = fp8;
     a.error_flag = gemm_error_flag(dev.index()).data_ptr<int>();
     a.wait_limit = gemm_wait_cycles(dev.index(), 2000.0);
-    const torch::Tensor scratch = torch::empty({(int64_t)dx::few_tokens_scratch(a)}, x.options().dtype(torch::kUInt8).requires_grad(false));
+    const torch::Tensor scratch = fresh({(int64_t)dx::few_tokens_scratch(a)}, at::kByte, x);
     a.scratch = scratch.data_ptr();
     launched(dx::launch_few_tokens(a, sms_of(x), stream_of(x)), what);
     return y;
@@ -278,6 +294,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
 
 void bind_block(py::module_& m) {
     m.def("rms_norm", &rms_norm);
+    m.def("rms_norm_fp8", &rms_norm_fp8);
     m.def("rms_norm_grad", &rms_norm_grad);
     m.def("rms_norm_bwd", &rms_norm_bwd);
     m.def("select_experts", &select_experts);

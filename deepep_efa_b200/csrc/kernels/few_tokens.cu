@@ -18,7 +18,7 @@
 // meet at the end, in a fixed order. So nothing is exchanged through memory but h, and no result depends on an order of arrival. The second launch begins
 // while the first one ends (programmatic dependent launch): it plans, fills its rings with weights, and only then waits for h.
 //
-// Types: e4m3 becomes fp16 in registers, exactly and with one instruction per pair (bf16 takes four: 8 tokens, FP8, us XXX), and each 128 x 128 block's sum is scaled in
+// Types: e4m3 becomes fp16 in registers, exactly and with one instruction per pair (bf16 takes four: 8 tokens, FP8, us 447 / 440), and each 128 x 128 block's sum is scaled in
 // fp32. Next to it activations are fp16 times a power of two per 128 of them. h has more bits than bf16, so that its rounding is small beside that of the result: next
 // to bf16 weights two bf16 numbers, a rounding and its remainder, whose products go to the same accumulators; next to e4m3 weights fp16 with a power of two per 16 values.
 #include <cuda.h>
@@ -666,8 +666,9 @@ cudaError_t launch_both(FewParams& p, int num_sms, cudaStream_t stream) {
     if (!make_weight_map(&up, a.w13, kFp8, true, a.experts, a.inter, a.hidden) || !make_weight_map(&down, a.w2, kFp8, false, a.experts, a.hidden, a.inter))
         return cudaErrorInvalidValue;
     const size_t up_smem = smem_bytes(true, 1), down_smem = smem_bytes(false, a.tokens);
+    constexpr size_t most_down = std::max(smem_bytes(false, 8), smem_bytes(false, kFewMaxTokens));
     cudaError_t e = cudaFuncSetAttribute(few_up_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)up_smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_down_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)down_smem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(few_down_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most_down);
     // No more CTAs than there can be units for: beside fewer than two per SM the second launch finds room at once.
     const long long units = (long long)std::min(a.tokens * a.topk, a.experts + a.tokens * a.topk / kCols) * ((a.inter + 15) / 16), teams = kWarps / kTeamWarps;
     const int up_ctas = (int)std::min<long long>(2 * num_sms, (units + teams - 1) / teams);

@@ -23,10 +23,10 @@ def few_token_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: tor
     (``H``, ``I`` multiples of 8), or e4m3 with fp32 scales per block of 128 x 128 (``MoELayer.prepare_fp8``; multiples of 128). Activations stay in bf16 in both
     cases: the hidden values, their weights included, are rounded to it once, sums are in fp32. Ids without an expert in ``[first_expert, first_expert + L)`` are
     skipped, so ranks that share the experts each compute their part of the sum. Forward only; no host synchronisation, so a step can be captured into a graph."""
-    if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or w13.requires_grad or w2.requires_grad):
-        raise ValueError("deepep_efa_b200.few_token_experts: forward only; call it under torch.no_grad()")
     if x.is_cuda:
         return _ext.load().few_tokens(x, topk_idx, topk_weights, w13, w2, w13_scales, w2_scales, first_expert, out)
+    if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or w13.requires_grad or w2.requires_grad):
+        raise ValueError("deepep_efa_b200.few_token_experts: forward only; call it under torch.no_grad()")
     if x.size(0) > MAX_TOKENS:
         raise ValueError("deepep_efa_b200.few_token_experts: at most 32 tokens")
     y = reference_few_token_experts(x, topk_idx, topk_weights, w13, w2, w13_scales, w2_scales, first_expert).to(x.dtype)

@@ -79,11 +79,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
 
     ``q`` e4m3 ``[N, H]`` and ``scales`` fp32 ``[N, H / 128]`` are made from the normed values in fp32 as the dispatch casts its rows (largest magnitude of 128
     channels, at least 1e-4, over 448; with ``round_scale`` rounded up to a power of two). ``y`` is bf16, None without ``keep_rows``; ``total`` is None without ``residual``."""
+    if x.is_cuda:
+        return _ext.load().rms_norm_fp8(x, weight, residual, eps, round_scale, keep_rows)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         raise ValueError("deepep_efa_b200.rms_norm_fp8: forward only; call it under torch.no_grad()")
-    if x.is_cuda:
-        y, q, scales, total = _ext.load().rms_norm(x, weight, residual, eps, keep_rows, True, round_scale)
-        return (q, scales), y, total
     _check_cpu(x, weight, residual)
     if x.dim() != 2 or x.size(1) % 128 != 0:
         raise ValueError("deepep_efa_b200.rms_norm_fp8: x must be [N, H] with H a multiple of 128")
