@@ -414,13 +414,21 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
         const int o = member * 32 + lane, r = o & 15, c = o >> 4, code = c < n ? s.pair[at + c] : 0, q = (code >> 5) * a.topk + (code & 31);
         const float first_weight = c < n ? a.weights[q] : 0.f;
         float acc[2][4] = {};
-        for (; j < boxes; j += kTeamWarps) {
-            constexpr int kPieces = kFp8 ? 4 : 2;
-            int4 b[kPieces], w[2][2][2];
+        constexpr int kPieces = kFp8 ? 4 : 2;
+        int4 b[kPieces];  // this lane's activations of a box; zeros all along where it has no column
 #pragma unroll
-            for (int i = 0; i < kPieces; ++i) {
-                const int k = j * kBoxK + (kFp8 ? (i >> 1) * 64 + t * 16 + (i & 1) * 8 : i * 32 + t * 8);
-                b[i] = mine >= 0 && k < a.hidden ? *reinterpret_cast<const int4*>(x + k) : make_int4(0, 0, 0, 0);
+        for (int i = 0; i < kPieces; ++i) b[i] = make_int4(0, 0, 0, 0);
+        for (; j < boxes; j += kTeamWarps) {
+            int4 w[2][2][2];
+            if (mine >= 0) {
+                const int4* from = reinterpret_cast<const int4*>(x + j * kBoxK + t * (kFp8 ? 16 : 8));
+                if constexpr (kFp8) {
+                    b[0] = from[0], b[1] = from[1], b[2 % kPieces] = from[8], b[3 % kPieces] = from[9];
+                } else {
+                    const int k = j * kBoxK + t * 8;
+                    b[0] = k < a.hidden ? from[0] : make_int4(0, 0, 0, 0);
+                    b[1] = k + 32 < a.hidden ? from[4] : make_int4(0, 0, 0, 0);
+                }
             }
             if constexpr (kFp8) {
                 const float gate = __ldg(scales + j), up = __ldg(scales + (long long)(a.inter / 128) * blocks_k + j);
@@ -552,6 +560,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
         }
     };
     const float* scales = nullptr;
+    int4 b[4];           // this lane's activations of a box, zeros all along where it has no column: four pieces of fp16, or [half of the box][rounding, remainder] in bf16
+    float hs[2];         // the powers of two of the two halves
     for (; now.b < end; advance(now)) {
         if (now.group != group) {
             if (group >= 0) flush();
@@ -559,14 +569,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
             at = s.group_start[group];
             n = (group + 1 < groups ? s.group_start[group + 1] : s.num_pairs) - at;
             mine = g < n ? (s.pair[at + g] >> 5) * a.topk + (s.pair[at + g] & 31) : -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) b[i] = make_int4(0, 0, 0, 0);
+            hs[0] = hs[1] = 1.f;
             if constexpr (kFp8) scales = a.s2 + ((long long)s.group_expert[group] * (a.hidden / 128) + tile * kBoxRows / 128) * (a.inter / 128);
         }
         int4 w[2][2][2];
         if constexpr (kFp8) {
-            int4 b[4];
-            float hs[2] = {1.f, 1.f};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) b[i] = make_int4(0, 0, 0, 0);
             const float scale = __ldg(scales + now.j);
             if (mine >= 0) {
                 const int4* h = reinterpret_cast<const int4*>(reinterpret_cast<const __half*>(p.h) + (long long)mine * a.inter + now.j * kBoxK + t * 16);
@@ -596,15 +605,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
                 for (int i = 0; i < 4; ++i) acc[m][i] = fmaf(col[i & 1], part[i], acc[m][i]);
             }
         } else {
-            int4 b[2][2];  // [half of the box][rounding, remainder]
-            const __nv_bfloat16* h = reinterpret_cast<const __nv_bfloat16*>(p.h) + (long long)mine * a.inter;
-            const long long plane = (long long)a.tokens * a.topk * a.inter;
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int k = now.j * kBoxK + c * 32 + t * 8;
-                const bool in = mine >= 0 && k < a.inter;
-                b[c][0] = in ? *reinterpret_cast<const int4*>(h + k) : make_int4(0, 0, 0, 0);
-                b[c][1] = in ? *reinterpret_cast<const int4*>(h + plane + k) : make_int4(0, 0, 0, 0);
+            if (mine >= 0) {
+                const int k = now.j * kBoxK + t * 8;
+                const int4* from = reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(p.h) + (long long)mine * a.inter + k);
+                const long long plane = (long long)a.tokens * a.topk * a.inter / 8;
+                const int4 none = make_int4(0, 0, 0, 0);
+                b[0] = k < a.inter ? from[0] : none, b[1] = k < a.inter ? from[plane] : none;
+                b[2] = k + 32 < a.inter ? from[4] : none, b[3] = k + 32 < a.inter ? from[4 + plane] : none;
             }
             read_box(ring.next(s.full[warp], &s.abort, p.limit), row, t, w);
             __syncwarp();
@@ -613,8 +620,8 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
             for (int m = 0; m < 2; ++m)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    multiply(acc[m], w[m][0][c], w[m][1][c], b[c][0]);
-                    multiply(acc[m], w[m][0][c], w[m][1][c], b[c][1]);
+                    multiply(acc[m], w[m][0][c], w[m][1][c], b[2 * c]);
+                    multiply(acc[m], w[m][0][c], w[m][1][c], b[2 * c + 1]);
                 }
         }
     }
