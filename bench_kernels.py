@@ -1,6 +1,6 @@
 """Micro-benchmark of the memory-bound helper kernels (one GPU): layout, standalone FP8 cast (plain, masked, scale atoms),
-scale-atom builders, expert-major plan / gathers, two-level bookkeeping, the training-step elementwise kernels, and the
-single-rank forms of the collective kernels of the fused MoE path (count exchange, expert-major dispatch, stage reduce,
+scale-atom builders, expert-major plan / gathers, two-level bookkeeping, the training-step elementwise kernels, the norm and the choice of
+the experts in front of a layer, the experts for a few tokens, and the single-rank forms of the collective kernels of the fused MoE path (count exchange, expert-major dispatch, stage reduce,
 barrier).
 
     python bench_kernels.py [--rows 32768] [--hidden 7168] [--iters 20] [--warmup 5] [--only NAME]
@@ -89,7 +89,24 @@ def main():
                        dtype=torch.int64, device="cuda")
     dst_rows = torch.empty_like(x)
 
+    # in front of a layer: norm of the residual stream, choice of the experts; and a decode step of 8 tokens through 64 experts in FP8
+    norm_w = torch.ones(H, device="cuda")
+    logits = torch.randn(M, E, device="cuda", generator=g)
+    sel_idx, sel_w = C.select_experts(logits, K, True)
+    few_n, few_i = 64, 2048
+    few_x, few_w = x[:8].contiguous(), torch.rand(8, K, device="cuda", generator=g)
+    few_idx = torch.rand(8, few_n, device="cuda", generator=g).topk(K, dim=-1).indices
+    w13 = torch.randn(few_n, 2 * few_i, H, device="cuda", generator=g, dtype=torch.bfloat16).to(torch.float8_e4m3fn)
+    w2 = torch.randn(few_n, H, few_i, device="cuda", generator=g, dtype=torch.bfloat16).to(torch.float8_e4m3fn)
+    s13, s2 = (torch.rand(few_n, n // 128, k // 128, device="cuda", generator=g) for n, k in ((2 * few_i, H), (H, few_i)))
+
     cases = {
+        "rms_norm_kernel": (lambda: C.rms_norm(x, norm_w, dst_rows, 1e-6, True, False, False), M * H * 8),
+        "rms_norm_kernel_fp8_rows": (lambda: C.rms_norm(x, norm_w, dst_rows, 1e-6, True, True, False), M * H * 9 + M * H // 128 * 4),
+        "rms_norm_bwd_kernel": (lambda: C.rms_norm_bwd(x, norm_w, dst_rows, None, 1e-6), M * H * 6),
+        "select_kernel": (lambda: C.select_experts(logits, K, True), M * (E * 4 + K * 12)),
+        "select_bwd_kernel": (lambda: C.select_experts_bwd(logits, sel_idx, sel_w, sel_w, True), M * (E * 4 + K * 16)),
+        "few_tokens_kernels": (lambda: C.few_tokens(few_x, few_idx, few_w, w13, w2, s13, s2, 0, None), int(few_idx.unique().numel()) * 3 * few_i * H),
         "em_notify_kernel": (lambda: C.em_notify(rts, notify_args, E, UNIT_ROWS), Tf * K * 8 + E * Tf * 4 // 8),
         "em_dispatch_kernel": (em_dispatch, Tf * K * (H * 2 + H + H // 128 * 4 + 4)),
         "stage_reduce_kernel": (lambda: C.stage_reduce(fw.stage, out_f, idxf, wf, E), Tf * K * H * 2 + Tf * H * 2),

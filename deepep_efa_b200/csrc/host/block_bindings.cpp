@@ -11,7 +11,7 @@
 
 namespace py = pybind11;
 
-torch::Tensor gemm_error_flag(int device);               // gemm_bindings.cpp
+int* gemm_error_word(int device);  // gemm_bindings.cpp
 long long gemm_wait_cycles(int device, double timeout_ms);
 
 namespace {
@@ -208,6 +208,11 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
     }
 };
 torch::autograd::variable_list rms_norm_grad(const torch::Tensor& x, const torch::Tensor& weight, const c10::optional<torch::Tensor>& residual, double eps) {
+    if (!at::GradMode::is_enabled() || !(x.requires_grad() || weight.requires_grad() || (residual.has_value() && residual->requires_grad()))) {
+        const auto [y, q, scales, total] = rms_norm(x, weight, residual, eps, true, false, false);
+        if (total.has_value()) return {*y, *total};
+        return {*y};
+    }
     return RMSNorm::apply(x, weight, residual, eps);
 }
 
@@ -282,7 +287,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     a.hidden = (int)H;
     a.inter = (int)I;
     a.fp8 = fp8;
-    a.error_flag = gemm_error_flag(dev.index()).data_ptr<int>();
+    a.error_flag = gemm_error_word(dev.index());
     a.wait_limit = gemm_wait_cycles(dev.index(), 2000.0);
     const torch::Tensor scratch = fresh({(int64_t)dx::few_tokens_scratch(a)}, at::kByte, x);
     a.scratch = scratch.data_ptr();

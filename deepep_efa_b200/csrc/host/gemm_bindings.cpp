@@ -22,11 +22,19 @@ namespace {
         if (!(cond)) throw std::invalid_argument(std::string("deepep_efa_b200.grouped_gemm: ") + (msg)); \
     } while (0)
 
+std::mutex error_flags_mutex;
+std::map<int, torch::Tensor>& error_flags() {
+    static std::map<int, torch::Tensor> flags;
+    return flags;
+}
+bool has_error_flag(int device) {
+    std::lock_guard<std::mutex> g(error_flags_mutex);
+    return error_flags().count(device) != 0;
+}
 // One error word per device: set by a kernel whose bounded pipeline wait ran out.
 torch::Tensor error_flag(int device) {
-    static std::mutex mu;
-    static std::map<int, torch::Tensor> flags;
-    std::lock_guard<std::mutex> g(mu);
+    auto& flags = error_flags();
+    std::lock_guard<std::mutex> g(error_flags_mutex);
     auto it = flags.find(device);
     if (it == flags.end()) {
         auto t = torch::zeros({1}, torch::TensorOptions().dtype(torch::kInt32).device(torch::kCUDA, device));
@@ -549,7 +557,11 @@ std::string bf16_form(int64_t rows, int64_t groups, int64_t n, int64_t k, bool m
 }
 
 // For the other kernels with bounded waits: the device's error word, and how many cycles a wait may take.
-torch::Tensor gemm_error_flag(int device) { return error_flag(device); }
+// (None yet, and a capture going on: a word made now would belong to the graph and be cleared by its replays, so there is none for this call.)
+int* gemm_error_word(int device) {
+    if (!has_error_flag(device) && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) return nullptr;
+    return error_flag(device).data_ptr<int>();
+}
 long long gemm_wait_cycles(int device, double timeout_ms) { return (long long)(timeout_ms * (double)clock_khz(device)); }
 
 void bind_gemm(py::module_& m) {

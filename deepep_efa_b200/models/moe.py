@@ -344,7 +344,7 @@ class MoELayer(nn.Module):
         if not fp8:
             return few_token_experts(x, topk_idx, topk_weights, self.w13, self.w2)
         if self._fp8 is None:
-            self.prepare_fp8()
+            self.prepare_fp8(native_block_scaling=x.is_cuda)
         (w13, s13), (w2, s2) = self._fp8
         return few_token_experts(x, topk_idx, topk_weights, w13, w2, w13_scales=s13, w2_scales=s2)
 

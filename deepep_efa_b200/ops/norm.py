@@ -62,6 +62,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     of ``x``'s shape ``(y, x + residual)``. Differentiable in all three; ``weight``'s gradient is summed in fp32 in a fixed order and has its type."""
     shape = x.shape
     if x.dim() != 2:
+        if residual is not None and residual.shape != shape:
+            raise ValueError("deepep_efa_b200.rms_norm: residual must be of x's shape")
         x, residual = x.reshape(-1, shape[-1]), None if residual is None else residual.reshape(-1, shape[-1])
     if x.is_cuda:
         out = _ext.load().rms_norm_grad(x, weight, residual, eps)
