@@ -459,3 +459,39 @@ def test_few_tokens_need_every_expert():
             layer.forward_few_tokens(_rows(2, 128, 1))
     finally:
         vc.destroy()
+
+
+def test_rows_far_apart():
+    """Rows whose last one begins past 2^31 elements: the norm and its gradients, the choice, the experts' tokens."""
+    rms_norm, _, select_experts, few = _ops()
+    room = torch.empty(300, 2 ** 23, dtype=torch.bfloat16, device="cuda")
+    parts = [room[:, at:at + 256] for at in (8, 512, 1024, 2048)]
+    for i, part in enumerate(parts):
+        part.copy_(_rows(300, 256, 20 + i))
+    w = _weight(256, True)
+    near = [p.contiguous() for p in parts]
+
+    def step(x, r, dy, dt):
+        x, r, c = x.detach().requires_grad_(), r.detach().requires_grad_(), w.detach().requires_grad_()
+        y, total = rms_norm(x, c, r)
+        return (y.detach(), total.detach(), *torch.autograd.grad((y, total), (x, r, c), (dy, dt)))
+    assert all(torch.equal(p, q) for p, q in zip(step(*parts), step(*near)))
+    assert all(torch.equal(p, q) for p, q in zip(select_experts(parts[0], 8), select_experts(near[0], 8)))
+    _, idx, weights, w13, w2, _, _ = refs.layer_inputs(32, 256, 64, 4, 2, False, "cuda")
+    assert torch.equal(few(parts[0][268:], idx, weights, w13, w2), few(near[0][268:], idx, weights, w13, w2))
+
+
+def test_experts_captured_first():
+    """A capture before anything else of the library ran on the device: its error word is not the graph's."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch, block_refs as refs; from deepep_efa_b200 import _ext; from deepep_efa_b200.ops.few_tokens import few_token_experts as few\n"
+            "v = refs.layer_inputs(3, 128, 128, 4, 2, True, 'cuda'); _ext.load(); torch.cuda.synchronize(); g = torch.cuda.CUDAGraph()\n"
+            "with torch.cuda.graph(g):\n    y = few(*v[:5], w13_scales=v[5], w2_scales=v[6])\n"
+            "g.replay(); torch.cuda.synchronize(); out, bound = refs.experts(*v)\n"
+            "assert ((y.double() - out).abs() <= bound).all() and _ext.load().gemm_error(0) == 0; print('fine')")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join((root, os.path.join(root, "tests"))))
+    done = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and "fine" in done.stdout, done.stderr[-2000:]
