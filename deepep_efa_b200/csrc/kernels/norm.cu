@@ -300,8 +300,7 @@ struct Shape {
 Shape shape_of(long long rows, int hidden, int num_sms) {
     const int n16 = (hidden + 7) / 8;
     // few rows: as many threads as there are chunks, for the shortest way through a row; many: several rows per SM at a time
-    const int most = rows <= num_sms ? 1024 : 256;
-    const int chunks = n16 <= most ? 1 : n16 <= 2 * most ? 2 : 4;
+    const int chunks = rows <= num_sms ? (n16 <= 1024 ? 1 : n16 <= 2048 ? 2 : 4) : (n16 >= 512 ? 4 : n16 >= 256 ? 2 : 1);
     return {chunks, ((n16 + chunks - 1) / chunks + 31) / 32 * 32};
 }
 
