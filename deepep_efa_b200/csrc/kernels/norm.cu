@@ -160,7 +160,7 @@ __device__ __forceinline__ void copy16(uint32_t to, const int4* from) {
 // A CTA takes every gridDim.x-th row and keeps its share of the weight's gradient in registers, and the weight, where rows are not too wide. A thread copies its own
 // chunks of the rows ahead into shared memory and reads them back alone, so that loads stay in flight over a row's sums without a barrier. Chunks past the
 // row's end, and a dtotal that is not there, are zeros in shared memory from the start. 8192 x 4096, us: row after row
-// straight to registers 62; rows ahead, 16 channels per thread 64; 32 per thread 60; math in pairs, weight kept 43 (its 268 MB at the measured copy rate: 41).
+// straight to registers 62; rows ahead, 16 channels per thread 64; 32 per thread 60; math in pairs, weight kept 43 (its 268 MB at the measured copy rate: 41). In a loop, with the weight's sum behind it, 45.
 template <int C, int S, int kMostThreads, bool kWide>
 __global__ void __launch_bounds__(kMostThreads) rms_norm_bwd_kernel(const NormBwdArgs a) {
     extern __shared__ __align__(16) uint8_t ahead[];  // [S][three arrays][C * threads chunks of 16 bytes]
@@ -317,12 +317,14 @@ struct BwdShape {
     size_t smem;
 };
 BwdShape bwd_shape_of(int hidden) {
-    // Many channels per thread: what a row costs a warp beside its channels (two sums over the CTA, addresses) was two thirds of the instructions with 16 of them.
-    const int n16 = (hidden + 7) / 8, chunks = n16 >= 512 ? 4 : n16 >= 256 ? 2 : 1;
+    // Many channels per thread: what a row costs a warp beside its channels (two sums over the CTA, addresses) was two thirds of the instructions with 16 of them. Few of a
+    // narrow row, whose CTAs are small enough anyway. us with 8 / 16 / 32 channels: 20000 x 1544 - / 58 / 55, 32768 x 1024 51 / 55 / 53, 70000 x 512 57 / 64 / -; 16384 x 2048 - / 53 / 50.
+    // Three rows ahead where six fit an SM: 8192 x 4096 with 4 x 2 / 3 x 3 rows 49.4 / 45.4, 8192 x 5120 with 3 x 2 / 2 x 3 59.8 / 58.7.
+    const int n16 = (hidden + 7) / 8, chunks = n16 >= 192 ? 4 : 1;
     BwdShape b;
     b.row = {chunks, ((n16 + chunks - 1) / chunks + 31) / 32 * 32};
     const size_t bytes = (size_t)3 * chunks * b.row.threads * 16, most = 220 * 1024;
-    b.stages = 12 * bytes <= most ? 3 : 2 * bytes <= most ? 2 : 1;
+    b.stages = 6 * bytes <= most ? 3 : 2 * bytes <= most ? 2 : 1;
     b.smem = b.stages * bytes;
     const int by_smem = (int)(most / (b.smem + 2048)), by_threads = (chunks == 4 ? 512 : 1024) / b.row.threads;
     b.per_sm = by_smem < by_threads ? by_smem : by_threads;
@@ -337,7 +339,6 @@ cudaError_t norm_backward_as(const NormBwdArgs& a, const BwdShape& b, int ctas, 
 template <bool kWide>
 cudaError_t norm_backward(const NormBwdArgs& a, const BwdShape& b, int ctas, cudaStream_t stream) {
     if (b.row.chunks == 1) return norm_backward_as<1, 3, 256, kWide>(a, b, ctas, stream);
-    if (b.row.chunks == 2) return norm_backward_as<2, 3, 256, kWide>(a, b, ctas, stream);
     if (b.row.threads <= 256) return b.stages == 3 ? norm_backward_as<4, 3, 256, kWide>(a, b, ctas, stream) : norm_backward_as<4, 2, 256, kWide>(a, b, ctas, stream);
     return b.stages == 2 ? norm_backward_as<4, 2, 1024, kWide>(a, b, ctas, stream) : norm_backward_as<4, 1, 1024, kWide>(a, b, ctas, stream);
 }
