@@ -123,30 +123,40 @@ __device__ __forceinline__ uint32_t to_half(uint32_t v, uint32_t under) {
     const __half2 r = __floats2half2_rn(f.x, f.y);
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// By all threads, four tokens at a time, while the first boxes are on their way. (A power of two per box and column instead took no such pass but 38 of a box's 320 instructions: 1, 8 and
-// 32 tokens, FP8, us 67.4 / 426 / 299, so 65.4 / 418 / 302.)
-__device__ __forceinline__ void find_largest(const FewTokensArgs& a, Plan& s) {
+// By all threads, four tokens and four pieces of each at a time, while the first boxes are on their way. (A power of two per box and column instead took no such pass but 38
+// of a box's 320 instructions: 1, 8 and 32 tokens, FP8, us 67.4 / 426 / 299, so 64.9 / 415 / 297.)
+__device__ __forceinline__ void find_largest(const FewTokensArgs& a, uint32_t* largest) {
+    constexpr int V = 4, U = 4;
     const int chunks = a.hidden / 8;
-    for (int t0 = 0; t0 < a.tokens; t0 += 4) {
-        __nv_bfloat162 most[4];
+#pragma unroll 1
+    for (int t0 = 0; t0 < a.tokens; t0 += V) {
+        __nv_bfloat162 most[V];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) most[v] = __float2bfloat162_rn(0.f);
-#pragma unroll 4
-        for (int i = threadIdx.x; i < chunks; i += kThreads) {
+        for (int v = 0; v < V; ++v) most[v] = __float2bfloat162_rn(0.f);
+#pragma unroll 1
+        for (int i0 = threadIdx.x; i0 < chunks; i0 += kThreads * U) {
+            int4 x[V][U];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-                if (t0 + v >= a.tokens) continue;
-                const int4 x = *(reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.x) + (t0 + v) * a.x_stride) + i);
-                const uint32_t w[4] = {(uint32_t)x.x, (uint32_t)x.y, (uint32_t)x.z, (uint32_t)x.w};
+            for (int v = 0; v < V; ++v)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) most[v] = __hmax2(most[v], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[q])));
-            }
+                for (int k = 0; k < U; ++k) {
+                    const int i = i0 + k * kThreads;
+                    x[v][k] = t0 + v < a.tokens && i < chunks ? *(reinterpret_cast<const int4*>(reinterpret_cast<const __nv_bfloat16*>(a.x) + (t0 + v) * a.x_stride) + i)
+                                                              : make_int4(0, 0, 0, 0);
+                }
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const uint32_t w[4] = {(uint32_t)x[v][k].x, (uint32_t)x[v][k].y, (uint32_t)x[v][k].z, (uint32_t)x[v][k].w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) most[v] = __hmax2(most[v], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&w[q])));
+                }
         }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-            if (t0 + v >= a.tokens) continue;
+        for (int v = 0; v < V; ++v) {
             const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(__low2float(most[v]), __high2float(most[v]))));
-            if (lane_id() == 0) atomicMax(s.largest + t0 + v, m);
+            if (lane_id() == 0 && t0 + v < a.tokens) atomicMax(largest + t0 + v, m);
         }
     }
     __syncthreads();
@@ -410,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
         ahead_j += kTeamWarps;
     };
     for (int i = 0; i < kStages; ++i) issue();
-    if constexpr (kFp8) find_largest(a, s);
+    if constexpr (kFp8) find_largest(a, s.largest);
     auto meet = [&] { asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(kTeamWarps * 32) : "memory"); };
 
     int j = member;
