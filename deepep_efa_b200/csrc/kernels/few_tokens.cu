@@ -578,11 +578,13 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    mine_sums[token * kBoxRows + ((m * 16 + r * 8 + row + 8 * token) & 31)] += acc[m][2 * r + i];
-                    acc[m][2 * r + i] = 0.f;
-                }
+                for (int r = 0; r < 2; ++r) mine_sums[token * kBoxRows + ((m * 16 + r * 8 + row + 8 * token) & 31)] += acc[m][2 * r + i];
         }
+        // Columns without a selection too: zeros times a weight (or a scale) that is no number are NaN, which the next group's selection in that column would get.
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[m][i] = 0.f;
     };
     const float* scales = nullptr;
     int4 b[4];           // this lane's activations of a box, zeros all along where it has no column: four pieces of fp16, or [half of the box][rounding, remainder] in bf16

@@ -1,0 +1,42 @@
+"""Norm, choice of the experts and experts for a few tokens on the GPU where numbers, gradients or calls are out of the ordinary (tolerances: block_refs.py)."""
+import pytest
+import torch
+
+import block_refs as refs
+from deepep_efa_b200.ops.few_tokens import few_token_experts
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- weights that are no numbers ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [2, 6, 32])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_experts_keep_a_bad_w2_to_its_tokens(tokens, fp8):
+    """NaN and infinity in one expert's W2 (or its scales) reach the results of this expert's tokens, in the rows that hold them, and nothing else: every other number
+    is that of finite weights, bit for bit. Experts have groups of different size, one after the other in a warp's run of boxes."""
+    x, idx, weights, w13, w2, s13, s2 = refs.layer_inputs(tokens, 512, 384, 7, 3, fp8, "cuda", seed=tokens)
+    idx[0] = torch.tensor([2, 3, 5], device="cuda")
+    idx[1:] = torch.where(idx[1:] == 2, torch.full_like(idx[1:], -1), idx[1:])  # expert 2 has one token, the next ones have more
+    run = lambda w2, s2: few_token_experts(x, idx, weights, w13, w2, w13_scales=s13, w2_scales=s2)  # noqa: E731
+    good = run(w2, s2)
+    cases = []
+    for e in range(7):
+        if fp8:
+            bad = w2.clone()
+            bad.view(torch.uint8)[e, 9, ::64] = 0x7F
+            cases.append((e, bad, s2, slice(9, 10)))
+            for v in (float("nan"), float("inf")):
+                scales = s2.clone()
+                scales[e, 1] = v
+                cases.append((e, w2, scales, slice(128, 256)))
+        else:
+            for v in (float("nan"), float("inf")):
+                bad = w2.clone()
+                bad[e, 9, ::64] = v
+                cases.append((e, bad, s2, slice(9, 10)))
+    for e, w, s, rows in cases:
+        y, hit = run(w, s), (idx == e).any(-1)
+        assert not torch.isfinite(y[hit][:, rows].float()).any()
+        keep = torch.ones(512, dtype=torch.bool, device="cuda")
+        keep[rows] = False
+        assert torch.equal(y[~hit], good[~hit]) and torch.equal(y[:, keep], good[:, keep]), (e, int((y[~hit] != good[~hit]).sum()))
