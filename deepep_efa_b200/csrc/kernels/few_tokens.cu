@@ -502,11 +502,12 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
             const float v = silu(gate) * up * weight;
             const long long to = (long long)q * a.inter + i;
             if constexpr (kFp8) {
-                // sixteen lanes have the sixteen values of a scale: the power of two at or below the largest
+                // sixteen lanes have the sixteen values of a scale: the power of two at or below the largest (of zeros the smallest there is, so that they do not count
+                // in the box's, which is the largest of eight)
                 float most = fabsf(v);
 #pragma unroll
                 for (int x16 = 8; x16 > 0; x16 >>= 1) most = fmaxf(most, __shfl_xor_sync((lane & 16) ? 0xffff0000u : 0xffffu, most, x16));
-                const int field = most > 0.f && most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23), 1), 253) : 127;
+                const int field = most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23), 1), 253) : 127;
                 reinterpret_cast<__half*>(p.h)[to] = __float2half(v * __uint_as_float((uint32_t)(254 - field) << 23));
                 if (r == 0) p.h_scale[to / 16] = __uint_as_float((uint32_t)field << 23);
             } else if (i < a.inter) {

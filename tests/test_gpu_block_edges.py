@@ -40,3 +40,17 @@ def test_experts_keep_a_bad_w2_to_its_tokens(tokens, fp8):
         keep = torch.ones(512, dtype=torch.bool, device="cuda")
         keep[rows] = False
         assert torch.equal(y[~hit], good[~hit]) and torch.equal(y[:, keep], good[:, keep]), (e, int((y[~hit] != good[~hit]).sum()))
+
+
+# ---- small values beside zeros ----------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [1, 6])
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-4, 1e-8])
+def test_experts_with_rows_of_zeros(tokens, size):
+    """Sixteen gate rows, sixteen up rows, or all but sixteen, that are zero (pruned, or padded to the multiple of 128) cost the others of their box nothing."""
+    for zero in (slice(0, 16), slice(112, 128), slice(384 + 32, 384 + 48), slice(16, 384)):
+        v = refs.layer_inputs(tokens, 256, 384, 4, 2, True, "cuda", seed=11)
+        v[0] *= size
+        v[3].view(torch.uint8)[:, zero] = 0
+        y = few_token_experts(*v[:5], w13_scales=v[5], w2_scales=v[6])
+        out, bound = refs.experts(*v)
+        assert ((y.double() - out).abs() <= bound).all(), ((y.double() - out).abs() / bound).max().item()
