@@ -503,17 +503,21 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
             const long long to = (long long)q * a.inter + i;
             if constexpr (kFp8) {
                 // sixteen lanes have the sixteen values of a scale: the power of two at or below the largest (of zeros the smallest there is, so that they do not count
-                // in the box's, which is the largest of eight)
+                // in the box's, which is the largest of eight; of infinities the largest, next to which finite values stay finite)
                 float most = fabsf(v);
 #pragma unroll
                 for (int x16 = 8; x16 > 0; x16 >>= 1) most = fmaxf(most, __shfl_xor_sync((lane & 16) ? 0xffff0000u : 0xffffu, most, x16));
-                const int field = most < INFINITY ? min(max((int)(__float_as_uint(most) >> 23), 1), 253) : 127;
-                reinterpret_cast<__half*>(p.h)[to] = __float2half(v * __uint_as_float((uint32_t)(254 - field) << 23));
-                if (r == 0) p.h_scale[to / 16] = __uint_as_float((uint32_t)field << 23);
+                const uint32_t field = exponent_field(__float_as_uint(most));
+                reinterpret_cast<__half*>(p.h)[to] = __float2half(v * __uint_as_float((254u - field) << 23));
+                if (r == 0) p.h_scale[to / 16] = __uint_as_float(field << 23);
             } else if (i < a.inter) {
-                const __nv_bfloat16 hi = __float2bfloat16(v);
+                // an infinity has no remainder (and infinity - infinity is NaN); a finite value that would round to one is cut off instead
+                __nv_bfloat16 hi = __float2bfloat16(v);
+                float rest = v - __bfloat162float(hi);
+                if (fabsf(rest) == INFINITY) hi = __float2bfloat16_rz(v), rest = v - __bfloat162float(hi);
+                if (fabsf(v) == INFINITY) rest = 0.f;
                 reinterpret_cast<__nv_bfloat16*>(p.h)[to] = hi;
-                reinterpret_cast<__nv_bfloat16*>(p.h)[to + (long long)a.tokens * a.topk * a.inter] = __float2bfloat16(v - __bfloat162float(hi));
+                reinterpret_cast<__nv_bfloat16*>(p.h)[to + (long long)a.tokens * a.topk * a.inter] = __float2bfloat16(rest);
             }
         }
         meet();

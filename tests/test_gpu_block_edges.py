@@ -54,3 +54,38 @@ def test_experts_with_rows_of_zeros(tokens, size):
         y = few_token_experts(*v[:5], w13_scales=v[5], w2_scales=v[6])
         out, bound = refs.experts(*v)
         assert ((y.double() - out).abs() <= bound).all(), ((y.double() - out).abs() / bound).max().item()
+
+
+# ---- infinite hidden values ---------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fp8", [False, True])
+def test_experts_with_an_infinite_hidden_value(fp8):
+    """gate * up past the largest float is an infinity, which the result has with the sign of its weight, whatever finite values of any size stand beside it; and
+    values between the largest bf16 and the largest float stay finite."""
+    H, inter = 128, 256
+    x = torch.zeros(2, H, dtype=torch.bfloat16, device="cuda")
+    x[0, 0] = x[1, 0] = 1e19
+    w13, w2 = torch.zeros(1, 2 * inter, H, device="cuda"), torch.zeros(1, H, inter, device="cuda")
+    w13[0, :, 0] = 2.0 ** -4         # (6e17)^2
+    w13[0, [40, inter + 40], 0] = 2  # (2e19)^2: infinite
+    w2[0] = -1
+    w2[0, :, 40] = 1
+    w2[0, ::2] *= -1
+    one = torch.ones(2, 1, device="cuda")
+    idx = torch.zeros(2, 1, dtype=torch.int64, device="cuda")
+    if fp8:
+        scales = dict(w13_scales=torch.ones(1, 2 * inter // 128, H // 128, device="cuda"), w2_scales=torch.ones(1, H // 128, inter // 128, device="cuda"))
+        a, b = w13.to(torch.float8_e4m3fn), w2.to(torch.float8_e4m3fn)
+    else:
+        scales, a, b = {}, w13.to(torch.bfloat16), w2.to(torch.bfloat16)
+    y = few_token_experts(x, idx, one, a, b, **scales).float()
+    assert (y[:, 0::2] == -torch.inf).all() and (y[:, 1::2] == torch.inf).all()
+    # one value alone, 2^128 (1 - 2^-10): a bf16 rounding of it would be infinite
+    w13.zero_()
+    w2.zero_()
+    w13[0, [3, inter + 3], 0] = 1
+    w2[0, :, 3] = 2.0 ** -6
+    x[:, 0] = 2.0 ** 63
+    a, b = w13.to(a.dtype), w2.to(b.dtype)
+    y = few_token_experts(x, idx, one * (4 * (1 - 2.0 ** -10)), a, b, **scales).double()
+    exact = 2.0 ** 122 * (1 - 2.0 ** -10)
+    assert ((y - exact).abs() <= (refs.BF16 + 2.0 ** -10) * exact).all()
