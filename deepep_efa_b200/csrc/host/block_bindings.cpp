@@ -2,12 +2,14 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <pybind11/functional.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
 #include <tuple>
 
 #include "../kernels/block_api.h"
+#include "../kernels/few_ring.h"
 
 namespace py = pybind11;
 
@@ -306,4 +308,15 @@ void bind_block(py::module_& m) {
     m.def("select_experts_grad", &select_experts_grad);
     m.def("select_experts_bwd", &select_experts_bwd);
     m.def("few_tokens", &few_tokens);
+    // (for tests without a GPU: what the warps of the experts for a few tokens keep of their rings)
+    py::class_<dx::RingState>(m, "FewTokensRing")
+        .def(py::init<int>())
+        .def("started", &dx::RingState::started)
+        .def("taken", &dx::RingState::taken)
+        .def("give_up", [](dx::RingState& r, const std::function<void(int, int)>& wait) { r.give_up(wait); })
+        .def_readonly("fill", &dx::RingState::fill)
+        .def_readonly("slot", &dx::RingState::slot)
+        .def_readonly("parity", &dx::RingState::parity)
+        .def_readonly("flying", &dx::RingState::flying)
+        .def_readonly("alive", &dx::RingState::alive);
 }

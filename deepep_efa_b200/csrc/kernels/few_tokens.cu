@@ -28,6 +28,7 @@
 #include <algorithm>
 
 #include "block_api.h"
+#include "few_ring.h"
 #include "launch.cuh"
 #include "tc_prims.cuh"
 
@@ -295,45 +296,28 @@ __device__ __forceinline__ void start_barriers(const CUtensorMap* map, Plan& s) 
 }
 
 // A warp's ring of boxes.
-struct Ring {
+struct Ring : RingState {
     uint32_t at, bars;
-    int stages, fill, slot, parity, flying;
-    bool alive;
-    __device__ __forceinline__ Ring(uint8_t* smem, Plan& s, int warp, int stages_) {
+    __device__ __forceinline__ Ring(uint8_t* smem, Plan& s, int warp, int stages_) : RingState(stages_) {
         at = smem_u32(smem) + warp * stages_ * kBoxBytes;
         bars = smem_u32(s.full[warp]);
-        stages = stages_;
-        fill = slot = parity = flying = 0;
-        alive = true;
     }
     __device__ __forceinline__ uint32_t fill_at() const { return at + fill * kBoxBytes; }
     __device__ __forceinline__ uint32_t fill_bar() const { return bars + fill * 8; }
-    __device__ __forceinline__ void filled() {
-        fill = fill + 1 == stages ? 0 : fill + 1;
-        ++flying;
-    }
-    // Waits for the next box; its place.
+    // Waits for the next box; its place. Where a copy did not come, here or in another warp, it waits (again with a limit) for all that are in flight, and from then
+    // on returns at once with a place that holds nothing.
     __device__ __forceinline__ uint32_t next(uint64_t* full, int* abort, long long limit) {
-        alive = __all_sync(0xffffffffu, mbar_wait(full + slot, parity, abort, limit)) && alive;
+        if (!__all_sync(0xffffffffu, mbar_wait(full + slot, parity, abort, limit)))
+            give_up([&](int i, int phase) {
+                const long long t0 = clock64();
+                while (!mbar_try_wait(full + i, phase) && clock64() - t0 < limit) {}
+            });
         const uint32_t box = at + slot * kBoxBytes;
-        if (++slot == stages) {
-            slot = 0;
-            parity ^= 1;
-        }
-        --flying;
+        taken();
         return box;
     }
-    // A copy did not come: waits for those in flight and says so.
-    __device__ __forceinline__ void give_up(uint64_t* full, int* error_flag, long long limit) {
-        for (; flying > 0; --flying) {
-            const long long t0 = clock64();
-            while (!mbar_try_wait(full + slot, parity) && clock64() - t0 < limit) {}
-            if (++slot == stages) {
-                slot = 0;
-                parity ^= 1;
-            }
-        }
-        if (lane_id() == 0 && error_flag != nullptr) atomicExch(error_flag, 1);
+    __device__ __forceinline__ void report(int* error_flag) const {
+        if (!alive && lane_id() == 0 && error_flag != nullptr) atomicExch(error_flag, 1);
     }
 };
 
@@ -416,7 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
             mbar_expect_tx_at(ring.fill_bar(), kBoxBytes);
             tma_load_box(&map, ring.fill_bar(), ring.fill_at(), ahead_j * kBoxK, ahead.block * 16, 0, e);
         }
-        ring.filled();
+        ring.started();
         ahead_j += kTeamWarps;
     };
     for (int i = 0; i < kStages; ++i) issue();
@@ -522,7 +506,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_up_kernel(const __grid_consta
         }
         meet();
     }
-    if (!ring.alive) ring.give_up(s.full[warp], a.error_flag, p.limit);
+    ring.report(a.error_flag);
 }
 
 // ---- second launch: W2 rows against h ---------------------------------------------------------------------------------------------------
@@ -563,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
             mbar_expect_tx_at(ring.fill_bar(), kBoxBytes);
             tma_load_box(&map, ring.fill_bar(), ring.fill_at(), ahead.j * kBoxK, tile * kBoxRows, e);
         }
-        ring.filled();
+        ring.started();
         advance(ahead);
     };
     for (int i = 0; i < stages; ++i) issue();
@@ -658,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, 2) few_down_kernel(const __grid_cons
         }
     }
     if (group >= 0) flush();
-    if (!ring.alive) ring.give_up(s.full[warp], a.error_flag, p.limit);
+    ring.report(a.error_flag);
     __syncthreads();
     // the warps' sums, in order, and then the cluster's
     const int outputs = a.tokens * kBoxRows;
