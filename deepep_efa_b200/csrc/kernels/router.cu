@@ -135,9 +135,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_bwd_kernel(const Select
             z += d[j];
         }
         z = warp_add(z);
-        const float f = z > 0.f ? -inner / z : 0.f;
+        // (no experts at all: zeros; a NaN among the logits is in Z and so in all entries, those of experts with -inf too)
+        const float f = z == 0.f ? 0.f : -inner / z;
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[j] = d[j] == 0.f ? 0.f : d[j] * f;
+        for (int j = 0; j < V; ++j) d[j] = d[j] == 0.f && z == z ? 0.f : d[j] * f;
     }
     const float at = w * (g - inner);
     for (int r = 0; r < a.topk; ++r) {

@@ -4,6 +4,7 @@ import torch
 
 import block_refs as refs
 from deepep_efa_b200.ops.few_tokens import few_token_experts
+from deepep_efa_b200.ops.router import select_experts
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,25 @@ def test_experts_with_an_infinite_hidden_value(fp8):
     y = few_token_experts(x, idx, one * (4 * (1 - 2.0 ** -10)), a, b, **scales).double()
     exact = 2.0 ** 122 * (1 - 2.0 ** -10)
     assert ((y - exact).abs() <= (refs.BF16 + 2.0 ** -10) * exact).all()
+
+
+# ---- gradient of a choice that has a NaN --------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_choice_gradient_with_nan(dtype):
+    """Probabilities among all experts are NaN in a row with a NaN, and so is every entry of its gradient; among the chosen ones, theirs. As on the CPU."""
+    logits = torch.randn(6, 40, generator=torch.Generator().manual_seed(1)).to(dtype)
+    logits[1, 7] = float("nan")
+    logits[2, 9] = float("inf")
+    logits[3, 5] = -float("inf")
+    logits[4, 5], logits[4, 30] = -float("inf"), float("nan")
+    dw = torch.randn(6, 3, generator=torch.Generator().manual_seed(2))
+    for renormalize in (False, True):
+        def gradient(device):
+            leaf = logits.to(device).requires_grad_()
+            _, weights = select_experts(leaf, 3, renormalize=renormalize)
+            return torch.autograd.grad(weights, leaf, dw.to(device))[0].cpu()
+        here, there = gradient("cuda"), gradient("cpu")
+        assert torch.equal(torch.isnan(here), torch.isnan(there))
+        if not renormalize:
+            assert torch.isnan(here[[1, 2, 4]]).all()
+        assert torch.isfinite(here[[0, 3, 5]].float()).all()
