@@ -212,24 +212,29 @@ class MoELayer(nn.Module):
 
     @torch.no_grad()
     def forward_fp8(self, x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], topk_idx: Optional[torch.Tensor] = None,
-                    topk_weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    topk_weights: Optional[torch.Tensor] = None, *, round_scale: Optional[bool] = None) -> torch.Tensor:
         """Forward only: FP8 on the wire and in both expert GEMMs, SwiGLU fused into the first GEMM, BF16 combine.
 
-        ``x`` may come quantised, as ``(e4m3 rows, fp32 scales per 128 channels)`` with its ids and weights (``rms_norm_fp8``; scales are powers of two
-        where ``prepare_fp8`` chose native block scaling)."""
+        ``x`` may come quantised, as ``(e4m3 rows, fp32 scales per 128 channels)`` with its ids and weights (``rms_norm_fp8``). Where ``prepare_fp8`` chose native block
+        scaling the scales have to be powers of two (``round_scale=True`` there), others are refused: pass the ``round_scale`` that the rows were made with, or
+        None to have the scales looked at, which the host waits for."""
         from .. import _ext
         C = _ext.load()
         if self._fp8 is None:
             self.prepare_fp8()
         (w13, s13), (w2, s2) = self._fp8
         quantised = isinstance(x, tuple)
-        if topk_idx is None:
-            if quantised:
+        mx = getattr(self, "_mx", None)
+        if quantised:
+            if topk_idx is None:
                 raise ValueError("deepep_efa_b200.forward_fp8: quantised rows come with their expert ids and weights")
+            # the tensor core takes a scale's exponent alone
+            if mx is not None and not (_powers_of_two(x[1]) if round_scale is None else round_scale):
+                raise ValueError("deepep_efa_b200.forward_fp8: native block scaling needs rows whose scales are powers of two (round_scale=True)")
+        elif topk_idx is None:
             topk_idx, topk_weights = self.route(x)
         num_tokens = x[0].size(0) if quantised else x.size(0)
         buf = self.buffer
-        mx = getattr(self, "_mx", None)
         per_rank, _, per_expert, in_rank, _ = buf.get_dispatch_layout(topk_idx, self.cfg.num_experts)
         (rx, rs), recv_idx, recv_w, counts, handle, _ = buf.dispatch(
             x, num_tokens_per_rank=per_rank, is_token_in_rank=in_rank, num_tokens_per_expert=per_expert, topk_idx=topk_idx,
@@ -368,8 +373,9 @@ class MoEBlock(nn.Module):
         """Prefill: the norm writes the rows that the dispatch sends (see :meth:`MoELayer.forward_fp8`)."""
         if self.moe._fp8 is None:
             self.moe.prepare_fp8()
-        rows, y, total = rms_norm_fp8(x, self.norm, residual, eps=self.eps, round_scale=getattr(self.moe, "_mx", None) is not None)
-        return self.moe.forward_fp8(rows, *self.moe.choose(y)), x if total is None else total
+        native = getattr(self.moe, "_mx", None) is not None
+        rows, y, total = rms_norm_fp8(x, self.norm, residual, eps=self.eps, round_scale=native)
+        return self.moe.forward_fp8(rows, *self.moe.choose(y), round_scale=native), x if total is None else total
 
     @torch.no_grad()
     def forward_few_tokens(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, fp8: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -407,6 +413,11 @@ FUSE_CAST_INTO_GEMM1 = True  # wide natively block-scaled tiles: GEMM1's epilogu
 # 538; 160 of 2560 -> 640, 135 rows, uniform, 387 / 362; FP8 layer, uniform: 128 of 2816 -> 896, 157 rows 499 / 414; 64 of 2304 -> 1280, 162 rows 333 / 298.
 SECOND_WINDOW_MIN_WEIGHT_BYTES = 400 << 20  # e4m3 bytes of this rank's experts
 SECOND_WINDOW_MIN_HIDDEN = 2304
+
+
+def _powers_of_two(scales: torch.Tensor) -> bool:
+    """Whether fp32 scales have nothing below their leading bit; the host waits for them. (Scales of other types are the dispatch's to refuse.)"""
+    return scales.dtype != torch.float32 or not bool((scales.view(torch.int32) & 0x7fffff).any())
 
 
 def _token_columns(rows: float, weight_bytes: int, hidden: int) -> int:

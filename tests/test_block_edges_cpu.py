@@ -1,7 +1,24 @@
 """What stands around the experts of a block where numbers or calls are out of the ordinary, without a GPU."""
+import types
+
 import pytest
+import torch
 
 from deepep_efa_b200 import _ext
+from deepep_efa_b200.models.moe import MoEConfig, MoELayer
+from deepep_efa_b200.ops.norm import rms_norm_fp8
+
+
+class Reached(Exception):
+    pass
+
+
+def lone_layer():
+    """A layer of a lone rank whose buffer says that it was reached."""
+    def layout(*_):
+        raise Reached
+    buffer = types.SimpleNamespace(group_size=1, rank=0, get_dispatch_layout=layout)
+    return MoELayer(MoEConfig(hidden=256, intermediate=128, num_experts=4, num_topk=2), buffer, device=torch.device("cpu"))
 
 
 # ---- a copy that does not come --------------------------------------------------------------------------------------------------------
@@ -35,3 +52,28 @@ def test_ring_of_a_warp_whose_wait_runs_out(stages, boxes):
                 start()
                 assert ring.flying == len(flying)
         assert ring.alive == (fails_at == boxes) and (not ring.alive or not flying) and ring.flying <= 0
+
+
+# ---- quantised rows and native block scaling ----------------------------------------------------------------------------------------------
+def test_quantised_rows_need_the_layers_scales():
+    """Native block scaling reads a scale's exponent alone: rows whose scales are no powers of two, or are not said to be, do not get as far as the dispatch."""
+    layer, w = lone_layer(), torch.ones(256)
+    layer.prepare_fp8(native_block_scaling=False)
+    x = torch.randn(5, 256, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    idx, weights = torch.zeros(5, 2, dtype=torch.int64), torch.ones(5, 2)
+    plain, powers = rms_norm_fp8(x, w)[0], rms_norm_fp8(x, w, round_scale=True)[0]
+    for rows in (plain, powers, (plain[0], plain[1].t().contiguous().t())):
+        for said in (None, False, True):  # fp32 scales of any kind
+            with pytest.raises(Reached):
+                layer.forward_fp8(rows, idx, weights, round_scale=said)
+    layer._mx = ()
+    for rows, said in ((powers, None), (powers, True), ((powers[0], powers[1].t().contiguous().t()), None), ((powers[0][:0], powers[1][:0]), None), (x, None)):
+        with pytest.raises(Reached):
+            layer.forward_fp8(rows, idx, weights, round_scale=said)
+    one = powers[1].clone()
+    one[3, 1] *= 1 + 2.0 ** -23
+    for rows, said in ((plain, None), (powers, False), ((powers[0], one), None)):
+        with pytest.raises(ValueError, match="powers of two"):
+            layer.forward_fp8(rows, idx, weights, round_scale=said)
+    with pytest.raises(ValueError, match="expert ids"):
+        layer.forward_fp8(powers)

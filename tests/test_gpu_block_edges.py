@@ -4,6 +4,7 @@ import torch
 
 import block_refs as refs
 from deepep_efa_b200.ops.few_tokens import few_token_experts
+from deepep_efa_b200.ops.norm import rms_norm, rms_norm_fp8
 from deepep_efa_b200.ops.router import select_experts
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +113,34 @@ def test_choice_gradient_with_nan(dtype):
         if not renormalize:
             assert torch.isnan(here[[1, 2, 4]]).all()
         assert torch.isfinite(here[[0, 3, 5]].float()).all()
+
+
+# ---- quantised rows and native block scaling ----------------------------------------------------------------------------------------------
+def test_quantised_rows_need_the_layers_scales():
+    """Native block scaling reads a scale's exponent alone. Rows whose scales are no powers of two are refused, found by looking or by what the caller says of them."""
+    from deepep_efa_b200.models.moe import MoEBlock, MoEConfig
+    from deepep_efa_b200.parallel.virtual import VirtualCluster
+    vc = VirtualCluster(1, num_nvl_bytes=64 << 20, num_rdma_bytes=0)
+    try:
+        block = MoEBlock(MoEConfig(hidden=256, intermediate=256, num_experts=8, num_topk=2, init_std=0.05), vc.buffers[0])
+        layer, w = block.moe, block.norm.detach()
+        x = torch.randn(40, 256, device="cuda").to(torch.bfloat16)
+        for native in (True, False):
+            layer.prepare_fp8(native_block_scaling=native)
+            (plain, y, _), (powers, _, _) = rms_norm_fp8(x, w), rms_norm_fp8(x, w, round_scale=True)
+            with torch.no_grad():
+                idx, weights = layer.choose(y)
+            want = layer.forward_fp8(y, idx, weights)
+            assert torch.equal(layer.forward_fp8(powers, idx, weights), layer.forward_fp8(powers, idx, weights, round_scale=True))
+            if native:
+                assert torch.equal(layer.forward_fp8(powers, idx, weights), block.forward_fp8(x)[0])
+                with pytest.raises(ValueError, match="powers of two"):
+                    layer.forward_fp8(plain, idx, weights)
+                with pytest.raises(ValueError, match="powers of two"):
+                    layer.forward_fp8(powers, idx, weights, round_scale=False)
+            else:
+                assert torch.equal(layer.forward_fp8(plain, idx, weights), block.forward_fp8(x)[0])
+            assert torch.isfinite(want.float()).all()
+        vc.buffers[0].check_status(sync=True)
+    finally:
+        vc.destroy()
