@@ -49,12 +49,19 @@ void forward_only(const char* what, std::initializer_list<const torch::Tensor*> 
     for (const torch::Tensor* t : tensors) DXB_CHECK(!t->requires_grad(), what, "forward only; call it under torch.no_grad()");
 }
 
+// There are no forward-mode derivatives, under no_grad either: refuses to drop a tangent silently, as autograd does for the CPU forms.
+void no_tangents(const char* what, std::initializer_list<const torch::Tensor*> tensors) {
+    for (const torch::Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "deepep_efa_b200.", what, ": no forward-mode derivative");
+}
+
 int sms_of(const torch::Tensor& t) { return at::cuda::getDeviceProperties(t.device().index())->multiProcessorCount; }
 
 // x [N, H] (+ residual) -> (y, q, scales, total), with None for what was not asked for
 std::tuple<c10::optional<torch::Tensor>, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>, c10::optional<torch::Tensor>> rms_norm(
     const torch::Tensor& x_in, const torch::Tensor& weight, c10::optional<torch::Tensor> residual, double eps, bool rows, bool quantize, bool round_scale) {
     const char* what = "rms_norm";
+    no_tangents(what, {&x_in, &weight, residual.has_value() ? &*residual : &x_in});
     DXB_CHECK(x_in.is_cuda() && x_in.dim() == 2 && x_in.scalar_type() == torch::kBFloat16, what, "x must be a CUDA bf16 matrix [N, H]");
     const int64_t N = x_in.size(0), H = x_in.size(1);
     DXB_CHECK(H > 0 && H % 8 == 0 && H <= dx::kNormMaxHidden, what, "hidden must be a multiple of 8, at most 32768");
@@ -152,6 +159,7 @@ torch::Tensor logit_rows(const torch::Tensor& t) { return t.size(1) == 1 || t.st
 
 std::tuple<torch::Tensor, torch::Tensor> select_experts(const torch::Tensor& logits_in, int64_t topk, bool renormalize) {
     const char* what = "select_experts";
+    no_tangents(what, {&logits_in});
     dx::SelectArgs a = select_args(what, logits_in, topk, renormalize);
     c10::cuda::CUDAGuard guard(logits_in.device());
     const torch::Tensor logits = logit_rows(logits_in);
@@ -244,6 +252,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     const char* what = "few_token_experts";
     const auto dev = x_in.device();
     forward_only(what, {&x_in, &weights_in, &w13, &w2});
+    no_tangents(what, {&x_in, &weights_in, &w13, &w2});
     DXB_CHECK(x_in.is_cuda() && x_in.dim() == 2 && x_in.scalar_type() == torch::kBFloat16, what, "x must be a CUDA bf16 matrix [T, H]");
     const int64_t T = x_in.size(0), H = x_in.size(1);
     DXB_CHECK(T <= dx::kFewMaxTokens, what, "at most 32 tokens");

@@ -144,3 +144,22 @@ def test_quantised_rows_need_the_layers_scales():
         vc.buffers[0].check_status(sync=True)
     finally:
         vc.destroy()
+
+
+# ---- tangents -----------------------------------------------------------------------------------------------------------------------------
+def test_forward_mode_is_refused():
+    """A tangent is not dropped without a word."""
+    import torch.autograd.forward_ad as fwd
+    x, w = torch.randn(4, 128, device="cuda").to(torch.bfloat16), torch.ones(128, device="cuda")
+    logits = torch.randn(4, 8, device="cuda")
+    v = refs.layer_inputs(3, 128, 128, 4, 2, False, "cuda")
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for bad in (lambda: rms_norm(dual(x), w), lambda: rms_norm(x, dual(w)), lambda: rms_norm(x, w, dual(x)), lambda: rms_norm_fp8(dual(x), w), lambda: rms_norm_fp8(x, w, dual(x)),
+                    lambda: select_experts(dual(logits), 2), lambda: few_token_experts(dual(v[0]), *v[1:5]), lambda: few_token_experts(*v[:2], dual(v[2]), *v[3:5]),
+                    lambda: few_token_experts(*v[:4], dual(v[4]))):
+            with pytest.raises(NotImplementedError):
+                bad()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                bad()
+        rms_norm(x, w), select_experts(logits, 2), few_token_experts(*v[:5])
