@@ -4,6 +4,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <pybind11/functional.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <tuple>
@@ -192,6 +194,17 @@ torch::Tensor select_experts_bwd(const torch::Tensor& logits_in, const torch::Te
     return dlogits;
 }
 
+// What a backward pass computed, where it was asked for with a graph: a node that refuses to be differentiated stands between it and `from`, what it depends on. Without
+// one second-order terms would be lost without a word.
+template <typename... T>
+torch::autograd::variable_list once(const char* what, torch::autograd::variable_list results, const T&... from) {
+    if (!at::GradMode::is_enabled() || !(from.requires_grad() || ...)) return results;
+    const auto refusal = std::make_shared<torch::autograd::Error>(std::string("deepep_efa_b200.") + what + ": the gradient is not differentiable",
+                                                                  torch::autograd::collect_next_edges(from...));
+    for (const auto& t : results) torch::autograd::set_history(t, refusal);
+    return results;
+}
+
 // The two with gradients as nodes of the autograd graph. In C++, since a step's launches are short: choice and gradient of 8192 x 64, us, as a Python function 70, so 58.
 struct RMSNorm : torch::autograd::Function<RMSNorm> {
     static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x, const torch::Tensor& weight,
@@ -207,14 +220,15 @@ struct RMSNorm : torch::autograd::Function<RMSNorm> {
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const bool residual = ctx->saved_data["residual"].toBool();
-        torch::Tensor dx, dw;
         c10::optional<torch::Tensor> past;
         if (residual && grads[1].defined()) past = grads[1];
-        if (grads[0].defined())
-            std::tie(dx, dw) = rms_norm_bwd(saved[0], saved[1], grads[0], past, ctx->saved_data["eps"].toDouble());
-        else if (past.has_value())
-            dx = *past;
-        return {dx, dw, residual ? dx : torch::Tensor(), torch::Tensor()};
+        if (!grads[0].defined()) {
+            const torch::Tensor dx = past.has_value() ? *past : torch::Tensor();
+            return {dx, torch::Tensor(), residual ? dx : torch::Tensor(), torch::Tensor()};
+        }
+        const auto [dx, dw] = rms_norm_bwd(saved[0], saved[1], grads[0], past, ctx->saved_data["eps"].toDouble());
+        const auto out = once("rms_norm", {dx, dw}, saved[0], saved[1], grads[0], past.has_value() ? *past : grads[0]);
+        return {out[0], out[1], residual ? out[0] : torch::Tensor(), torch::Tensor()};
     }
 };
 torch::autograd::variable_list rms_norm_grad(const torch::Tensor& x, const torch::Tensor& weight, const c10::optional<torch::Tensor>& residual, double eps) {
@@ -237,9 +251,9 @@ struct SelectExperts : torch::autograd::Function<SelectExperts> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        torch::Tensor dlogits;
-        if (grads[1].defined()) dlogits = select_experts_bwd(saved[0], saved[1], saved[2], grads[1], ctx->saved_data["renormalize"].toBool());
-        return {dlogits, torch::Tensor(), torch::Tensor()};
+        if (!grads[1].defined()) return {torch::Tensor(), torch::Tensor(), torch::Tensor()};
+        const torch::Tensor dlogits = select_experts_bwd(saved[0], saved[1], saved[2], grads[1], ctx->saved_data["renormalize"].toBool());
+        return {once("select_experts", {dlogits}, saved[0], grads[1])[0], torch::Tensor(), torch::Tensor()};
     }
 };
 std::tuple<torch::Tensor, torch::Tensor> select_experts_grad(const torch::Tensor& logits, int64_t topk, bool renormalize) {

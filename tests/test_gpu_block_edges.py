@@ -163,3 +163,35 @@ def test_forward_mode_is_refused():
             with torch.no_grad(), pytest.raises(NotImplementedError):
                 bad()
         rms_norm(x, w), select_experts(logits, 2), few_token_experts(*v[:5])
+
+
+# ---- second derivatives -------------------------------------------------------------------------------------------------------------------
+def test_second_derivatives_are_refused():
+    """Gradients that were asked for with a graph have one that says so; those that need none are as ever."""
+    x, w = torch.randn(4, 128, device="cuda").to(torch.bfloat16).requires_grad_(), torch.ones(128, device="cuda", requires_grad=True)
+    dy = torch.randn(4, 128, device="cuda").to(torch.bfloat16)
+    for residual in (None, x):
+        out = rms_norm(x, w, residual)
+        y = out if residual is None else out[0]
+        plain = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+        kept = torch.autograd.grad(y, (x, w), dy, create_graph=True)
+        assert all(torch.equal(a, b.detach()) and not a.requires_grad and b.requires_grad for a, b in zip(plain, kept))
+        for g, leaf in ((kept[0], x), (kept[0], w), (kept[1], x)):
+            with pytest.raises(RuntimeError, match="differentiable"):
+                torch.autograd.grad(g.float().square().sum(), leaf, retain_graph=True)
+        # beside a term that is twice differentiable it would be lost in silence
+        with pytest.raises(RuntimeError, match="differentiable"):
+            ((kept[0].float() + x.float().square()).sum()).backward(inputs=[x])
+        with pytest.raises(RuntimeError, match="differentiable"):
+            torch.autograd.grad((kept[1].float() + w.square()).sum(), w, retain_graph=True)
+    _, total = rms_norm(x, w, x)
+    (past,) = torch.autograd.grad(total, x, dy, create_graph=True)  # (a sum alone is linear)
+    assert torch.equal(past.detach(), dy + dy)
+    logits = torch.randn(5, 8, device="cuda", requires_grad=True)
+    for renormalize in (False, True):
+        _, weights = select_experts(logits, 2, renormalize=renormalize)
+        dw = torch.randn(5, 2, device="cuda")
+        plain, kept = (torch.autograd.grad(weights, logits, dw, retain_graph=True, create_graph=c)[0] for c in (False, True))
+        assert torch.equal(plain, kept.detach())
+        with pytest.raises(RuntimeError, match="differentiable"):
+            torch.autograd.grad(kept.square().sum(), logits)
