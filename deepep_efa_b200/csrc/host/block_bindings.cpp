@@ -265,7 +265,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
                          c10::optional<torch::Tensor> s13, c10::optional<torch::Tensor> s2, int64_t first, c10::optional<torch::Tensor> out) {
     const char* what = "few_token_experts";
     const auto dev = x_in.device();
-    forward_only(what, {&x_in, &weights_in, &w13, &w2});
+    forward_only(what, {&x_in, &weights_in, &w13, &w2, out.has_value() ? &*out : &x_in});
     no_tangents(what, {&x_in, &weights_in, &w13, &w2});
     DXB_CHECK(x_in.is_cuda() && x_in.dim() == 2 && x_in.scalar_type() == torch::kBFloat16, what, "x must be a CUDA bf16 matrix [T, H]");
     const int64_t T = x_in.size(0), H = x_in.size(1);
@@ -317,6 +317,7 @@ torch::Tensor few_tokens(const torch::Tensor& x_in, const torch::Tensor& idx_in,
     const torch::Tensor scratch = fresh({(int64_t)dx::few_tokens_scratch(a)}, at::kByte, x);
     a.scratch = scratch.data_ptr();
     launched(dx::launch_few_tokens(a, sms_of(x), stream_of(x)), what);
+    if (out.has_value() && !out->is_inference()) torch::autograd::impl::bump_version(*out);  // a graph that has kept `out` notices
     return y;
 }
 

@@ -195,3 +195,17 @@ def test_second_derivatives_are_refused():
         assert torch.equal(plain, kept.detach())
         with pytest.raises(RuntimeError, match="differentiable"):
             torch.autograd.grad(kept.square().sum(), logits)
+
+
+# ---- a result in a tensor that a graph has kept ----------------------------------------------------------------------------------------------
+def test_experts_into_a_tensor_that_was_kept_for_a_gradient():
+    v = refs.layer_inputs(3, 128, 128, 4, 2, False, "cuda")
+    out, leaf = torch.ones(3, 128, dtype=torch.bfloat16, device="cuda"), torch.ones(3, 128, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    kept = (out * leaf).sum()
+    few_token_experts(*v[:5], out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    with pytest.raises(ValueError, match="forward only"):
+        few_token_experts(*v[:5], out=leaf)
+    with torch.inference_mode():
+        few_token_experts(*v[:5], out=torch.empty(3, 128, dtype=torch.bfloat16, device="cuda"))
