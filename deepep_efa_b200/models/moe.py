@@ -340,8 +340,9 @@ class MoELayer(nn.Module):
     @torch.no_grad()
     def forward_few_tokens(self, x: torch.Tensor, topk_idx: Optional[torch.Tensor] = None, topk_weights: Optional[torch.Tensor] = None, fp8: bool = True) -> torch.Tensor:
         """Forward only, up to 32 tokens, on a rank that holds every expert: no dispatch, no combine, no host synchronisation (see
-        :func:`few_token_experts`). ``fp8=True`` reads the e4m3 weights (``prepare_fp8``), ``False`` the bf16 parameters; activations keep 16 bits either way, so results are
-        nearer to the bf16 layer than those of the paths that send e4m3 rows."""
+        :func:`few_token_experts`). ``fp8=True`` reads the e4m3 weights, ``False`` the bf16 parameters; activations keep 16 bits either way, so results are
+        nearer to the bf16 layer than those of the paths that send e4m3 rows. The first call makes the e4m3 weights if ``prepare_fp8`` has not (not in a capture: call
+        it before); after a change of the parameters call ``prepare_fp8`` again."""
         if self.buffer.group_size != 1:
             raise ValueError("deepep_efa_b200.forward_few_tokens: this rank holds a part of the experts; use forward_low_latency")
         if topk_idx is None:
@@ -349,6 +350,9 @@ class MoELayer(nn.Module):
         if not fp8:
             return few_token_experts(x, topk_idx, topk_weights, self.w13, self.w2)
         if self._fp8 is None:
+            if x.is_cuda and torch.cuda.is_current_stream_capturing():
+                # (they would hold nothing until the graph's first replay, and each replay would quantise them again)
+                raise ValueError("deepep_efa_b200.forward_few_tokens: call prepare_fp8 before a capture")
             self.prepare_fp8(native_block_scaling=x.is_cuda)
         (w13, s13), (w2, s2) = self._fp8
         return few_token_experts(x, topk_idx, topk_weights, w13, w2, w13_scales=s13, w2_scales=s2)

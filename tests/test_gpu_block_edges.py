@@ -1,4 +1,6 @@
 """Norm, choice of the experts and experts for a few tokens on the GPU where numbers, gradients or calls are out of the ordinary (tolerances: block_refs.py)."""
+import types
+
 import pytest
 import torch
 
@@ -209,3 +211,25 @@ def test_experts_into_a_tensor_that_was_kept_for_a_gradient():
         few_token_experts(*v[:5], out=leaf)
     with torch.inference_mode():
         few_token_experts(*v[:5], out=torch.empty(3, 128, dtype=torch.bfloat16, device="cuda"))
+
+
+# ---- weights that are quantised on the way -------------------------------------------------------------------------------------------------
+def test_few_tokens_are_not_captured_before_the_weights_are_quantised():
+    """Weights quantised inside a capture would hold nothing until its first replay, and be quantised again by each."""
+    from deepep_efa_b200.models.moe import MoEBlock, MoEConfig
+    buffer = types.SimpleNamespace(group_size=1, rank=0)
+    block = MoEBlock(MoEConfig(hidden=128, intermediate=128, num_experts=4, num_topk=2), buffer, device=torch.device("cuda"))
+    x = torch.randn(3, 128, device="cuda").to(torch.bfloat16)
+    block.forward_few_tokens(x, fp8=False)  # (what libraries make on their first call)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="prepare_fp8"):
+        with torch.cuda.graph(graph):
+            block.forward_few_tokens(x)
+    assert block.moe._fp8 is None
+    want = block.forward_few_tokens(x)[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = block.forward_few_tokens(x)[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
