@@ -6,8 +6,9 @@
 //                                   bf16 first would round twice.
 //   dtotal = r (weight dy - total r^2 mean(weight dy total)) + (what reaches the sum past the norm);   dweight = sum over rows of dy total r
 //
-// Sums are in fp32. Memory bound: a row is read once and stays in registers between its sum and its output. The gradient of the weight goes through one
-// partial sum per CTA and is added up in a fixed order, so results do not change from run to run.
+// Sums are in fp32. The squares of a row past some 2^59 are no floats, and its gradient's r^3 is none past 2^42: such rows are multiplied by 2^-80 (exact in bf16, but for what
+// is too small to count) and summed again, so a row's size does not matter. Memory bound: a row is read once and stays in registers between its sum and its output. The
+// gradient of the weight goes through one partial sum per CTA and is added up in a fixed order, so results do not change from run to run.
 #include "block_api.h"
 #include "launch.cuh"
 
@@ -41,6 +42,10 @@ __device__ __forceinline__ float warp_add(float v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+
+constexpr float kDown = 8.2718061255302767e-25f;       // 2^-80
+constexpr float kLargeSum = 1.2676506002282294e30f;    // 2^100, of a thread's squares in the forward pass
+constexpr float kLargeMean = 1.2089258196146292e24f;   // 2^80, of a row's squares in the gradient
 
 // One row per CTA, C chunks of eight channels per thread.
 template <int C, bool kWide>
@@ -86,11 +91,25 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
     }
+    // A warp with large values sums their squares times 2^-160 and says so by the sign.
+    const bool large = __any_sync(0xffffffffu, sum > kLargeSum);
+    if (large) {
+        sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float f[8];
+            unpack8(v[c], f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum = fmaf(f[j] * kDown, f[j] * kDown, sum);
+        }
+    }
     sum = warp_add(sum);
-    if (lane == 0) s_sum[tid >> 5] = sum;
+    if (lane == 0) s_sum[tid >> 5] = large ? -sum : sum;
     __syncthreads();
-    sum = warp_add(lane < threads / 32 ? s_sum[lane] : 0.f);
-    const float r = rsqrtf(sum / (float)a.hidden + a.eps);
+    const float part = lane < threads / 32 ? s_sum[lane] : 0.f;
+    sum = warp_add(part < 0.f ? 0.f : part);
+    float r = rsqrtf(sum / (float)a.hidden + a.eps);
+    if (__any_sync(0xffffffffu, part < 0.f)) r = kDown * rsqrtf(fmaf(sum, kDown * kDown, warp_add(part < 0.f ? -part : 0.f)) / (float)a.hidden + a.eps * kDown * kDown);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int i = c * threads + tid;
@@ -155,6 +174,14 @@ __device__ __forceinline__ void load_weight8(const void* w, int chunk, f32x2 (&f
 }
 __device__ __forceinline__ void copy16(uint32_t to, const int4* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
+__device__ __forceinline__ int4 scaled_down(const int4& v) {
+    float f[8];
+    unpack8(v, f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= kDown;
+    return pack8(f);
 }
 
 // A CTA takes every gridDim.x-th row and keeps its share of the weight's gradient in registers, and the weight, where rows are not too wide. A thread copies its own
@@ -227,34 +254,76 @@ __global__ void __launch_bounds__(kMostThreads) rms_norm_bwd_kernel(const NormBw
                 inner2 = fma2(mul2(g[j], w[j]), f[j], inner2);
             }
         }
-        float squares = warp_add(of_pair(squares2).x + of_pair(squares2).y), inner = warp_add(of_pair(inner2).x + of_pair(inner2).y);
-        if (lane == 0) s_sum[parity][tid >> 5] = make_float2(squares, inner);
-        __syncthreads();  // (two buffers: a warp that is a row ahead writes the other one)
-        squares = inner = 0.f;
-        for (int w = 0; w < threads / 32; ++w) {
-            const float2 part = s_sum[parity][w];
-            squares += part.x;
-            inner += part.y;
-        }
-        const float r = rsqrtf(fmaf(squares, per_channel, a.eps)), back = -r * r * r * (inner * per_channel);
-        const f32x2 r2 = pair_of(r, r), back2 = pair_of(back, back);
-        int4* o = reinterpret_cast<int4*>(a.dx) + row * n16 + tid;
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-            f32x2 f[4], g[4], w[4], u[4];
-            unpack8(now[c * threads], f);
-            unpack8(now[pitch + c * threads], g);
-            unpack8(now[2 * pitch + c * threads], u);
-            weight_of(c, w);
-            uint32_t out[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x2 gr = mul2(g[j], r2);
-                dw[c][j] = fma2(gr, f[j], dw[c][j]);
-                const float2 v = of_pair(fma2(gr, w[j], fma2(back2, f[j], u[j])));
-                out[j] = f2_to_bf16x2(v.x, v.y);
+        float squares = of_pair(squares2).x + of_pair(squares2).y, inner = of_pair(inner2).x + of_pair(inner2).y;
+        auto sum_over_row = [&] {
+            squares = warp_add(squares);
+            inner = warp_add(inner);
+            if (lane == 0) s_sum[parity][tid >> 5] = make_float2(squares, inner);
+            __syncthreads();  // (two buffers: a warp that is a row ahead writes the other one)
+            squares = inner = 0.f;
+            for (int w = 0; w < threads / 32; ++w) {
+                const float2 part = s_sum[parity][w];
+                squares += part.x;
+                inner += part.y;
             }
-            if (c * threads + tid < n16) st_once(o + c * threads, make_int4((int)out[0], (int)out[1], (int)out[2], (int)out[3]));
+        };
+        sum_over_row();
+        int4* o = reinterpret_cast<int4*>(a.dx) + row * n16 + tid;
+        if (squares * per_channel > kLargeMean) {  // (the same in all threads)
+            squares = inner = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < C; ++c) {
+                float f[8], g[8], w[8];
+                unpack8(scaled_down(now[c * threads]), f);
+                unpack8(now[pitch + c * threads], g);
+                load_weight8<kWide>(a.weight, c * threads + tid < n16 ? c * threads + tid : 0, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    squares = fmaf(f[j], f[j], squares);
+                    inner = fmaf(g[j] * w[j], f[j], inner);
+                }
+            }
+            __syncthreads();
+            sum_over_row();
+            const float r = rsqrtf(fmaf(squares, per_channel, a.eps * kDown * kDown)), back = -(r * r) * (r * (inner * per_channel));
+            const f32x2 r2 = pair_of(r, r), back2 = pair_of(back, back), down2 = pair_of(kDown, kDown);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                f32x2 f[4], g[4], w[4], u[4];
+                unpack8(scaled_down(now[c * threads]), f);
+                unpack8(now[pitch + c * threads], g);
+                unpack8(now[2 * pitch + c * threads], u);
+                weight_of(c, w);
+                uint32_t out[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 gr = mul2(g[j], r2);
+                    dw[c][j] = fma2(gr, f[j], dw[c][j]);
+                    const float2 v = of_pair(fma2(down2, fma2(gr, w[j], mul2(back2, f[j])), u[j]));
+                    out[j] = f2_to_bf16x2(v.x, v.y);
+                }
+                if (c * threads + tid < n16) o[c * threads] = make_int4((int)out[0], (int)out[1], (int)out[2], (int)out[3]);
+            }
+        } else {
+            const float r = rsqrtf(fmaf(squares, per_channel, a.eps)), back = -r * r * r * (inner * per_channel);
+            const f32x2 r2 = pair_of(r, r), back2 = pair_of(back, back);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                f32x2 f[4], g[4], w[4], u[4];
+                unpack8(now[c * threads], f);
+                unpack8(now[pitch + c * threads], g);
+                unpack8(now[2 * pitch + c * threads], u);
+                weight_of(c, w);
+                uint32_t out[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x2 gr = mul2(g[j], r2);
+                    dw[c][j] = fma2(gr, f[j], dw[c][j]);
+                    const float2 v = of_pair(fma2(gr, w[j], fma2(back2, f[j], u[j])));
+                    out[j] = f2_to_bf16x2(v.x, v.y);
+                }
+                if (c * threads + tid < n16) st_once(o + c * threads, make_int4((int)out[0], (int)out[1], (int)out[2], (int)out[3]));
+            }
         }
         fetch(row + (long long)S * gridDim.x, stage);
         stage = stage + 1 == S ? 0 : stage + 1;
@@ -340,7 +409,8 @@ template <bool kWide>
 cudaError_t norm_backward(const NormBwdArgs& a, const BwdShape& b, int ctas, cudaStream_t stream) {
     if (b.row.chunks == 1) return norm_backward_as<1, 3, 256, kWide>(a, b, ctas, stream);
     if (b.row.threads <= 256) return b.stages == 3 ? norm_backward_as<4, 3, 256, kWide>(a, b, ctas, stream) : norm_backward_as<4, 2, 256, kWide>(a, b, ctas, stream);
-    return b.stages == 2 ? norm_backward_as<4, 2, 1024, kWide>(a, b, ctas, stream) : norm_backward_as<4, 1, 1024, kWide>(a, b, ctas, stream);
+    // Two stages fit where a row has at most 576 threads, which leaves each 96 registers (us with 64: 3000 x 9000 111, so 97; 2000 x 16384 82, so 73).
+    return b.stages == 2 ? norm_backward_as<4, 2, 576, kWide>(a, b, ctas, stream) : norm_backward_as<4, 1, 1024, kWide>(a, b, ctas, stream);
 }
 
 }  // namespace

@@ -28,6 +28,13 @@ def _check_cpu(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.T
         raise ValueError("deepep_efa_b200.rms_norm: residual must be of x's shape and type")
 
 
+def _sized(t: torch.Tensor, eps: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(rows, 1 / sqrt(mean square + eps) of them, the power of two that they were multiplied with)``: large rows, whose squares are no floats, are made small first."""
+    down = torch.where(t.abs().amax(-1, keepdim=True) > 2.0 ** 40, 2.0 ** -80, 1.0)
+    t = t * down
+    return t, torch.rsqrt(t.square().mean(-1, keepdim=True) + eps * down * down), down
+
+
 class _RMSNorm(torch.autograd.Function):
     """The CPU form."""
 
@@ -37,8 +44,8 @@ class _RMSNorm(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         _check_cpu(x, weight, residual)
         total = None if residual is None else _total(x, residual)
-        t = (x if residual is None else total).float()
-        y = (t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()).to(x.dtype)
+        t, r, _ = _sized((x if residual is None else total).float(), eps)
+        y = (t * r * weight.float()).to(x.dtype)
         ctx.save_for_backward(x if residual is None else total, weight)
         return y if residual is None else (y, total)
 
@@ -48,10 +55,9 @@ class _RMSNorm(torch.autograd.Function):
         if dy is None:
             dx, dw = dtotal, None
         else:
-            t, g = total.float(), dy.float()
-            r = torch.rsqrt(t.square().mean(-1, keepdim=True) + ctx.eps)
+            (t, r, down), g = _sized(total.float(), ctx.eps), dy.float()
             wg = g * weight.float()
-            dx = r * (wg - t * r * r * (wg * t).mean(-1, keepdim=True))
+            dx = down * (r * (wg - t * r * r * (wg * t).mean(-1, keepdim=True)))
             dx = (dx if dtotal is None else dx + dtotal.float()).to(total.dtype)
             dw = (g * t * r).sum(0).to(weight.dtype)
         return dx, dw, dx if ctx.has_residual else None, None
@@ -59,7 +65,7 @@ class _RMSNorm(torch.autograd.Function):
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
     """The norm of the rows of ``x`` (bf16 ``[..., H]``, ``H`` a multiple of 8 up to 32768; ``weight`` bf16 or fp32 ``[H]``). Returns ``y``, or with a ``residual``
-    of ``x``'s shape ``(y, x + residual)``. Differentiable in all three; ``weight``'s gradient is summed in fp32 in a fixed order and has its type."""
+    of ``x``'s shape ``(y, x + residual)``. A row's size does not matter, up to the largest bf16. Differentiable in all three, once; ``weight``'s gradient is summed in fp32 in a fixed order and has its type."""
     shape = x.shape
     if x.dim() != 2:
         if residual is not None and residual.shape != shape:
@@ -89,8 +95,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     if x.dim() != 2 or x.size(1) % 128 != 0:
         raise ValueError("deepep_efa_b200.rms_norm_fp8: x must be [N, H] with H a multiple of 128")
     total = _total(x, residual)
-    t = total.float()
-    v = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + eps) * weight.float()
+    t, r, _ = _sized(total.float(), eps)
+    v = t * r * weight.float()
     amax = v.view(v.size(0), -1, 128).abs().amax(-1).clamp(min=1e-4)
     scales, inv = amax / 448.0, 448.0 / amax
     if round_scale:

@@ -4,9 +4,10 @@ import types
 import pytest
 import torch
 
+import block_refs as refs
 from deepep_efa_b200 import _ext
 from deepep_efa_b200.models.moe import MoEConfig, MoELayer
-from deepep_efa_b200.ops.norm import rms_norm_fp8
+from deepep_efa_b200.ops.norm import rms_norm, rms_norm_fp8
 
 
 class Reached(Exception):
@@ -77,3 +78,27 @@ def test_quantised_rows_need_the_layers_scales():
             layer.forward_fp8(rows, idx, weights, round_scale=said)
     with pytest.raises(ValueError, match="expert ids"):
         layer.forward_fp8(powers)
+
+
+# ---- rows whose squares are no floats ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("wide", [False, True])
+def test_norm_of_large_rows(wide):
+    """Rows from 2^10 to the largest bf16 beside ordinary ones: the norm does not depend on a row's size, and neither do the bounds."""
+    g = torch.Generator().manual_seed(7)
+    x, dy, dt = (torch.randn(40, 256, generator=g).to(torch.bfloat16) for _ in range(3))
+    for i, power in enumerate((10, 30, 39, 40, 41, 42, 58, 59, 60, 61, 63, 64, 80, 120, 124)):
+        x[2 * i] *= 2.0 ** power
+    x[39, 1:], x[39, 0] = 0, 3e38
+    dt[::4] = 0
+    x.requires_grad_()
+    w = (1 + 0.2 * torch.randn(256, generator=g)).to(torch.float32 if wide else torch.bfloat16).requires_grad_()
+    y, total = rms_norm(x, w, torch.zeros_like(x))
+    exact, _ = refs.norm(x.detach(), w.detach(), 1e-6)
+    assert torch.equal(total, x) and ((y.double() - exact).abs() <= (refs.BF16 + refs.NORM) * exact.abs()).all()
+    gx, gw = torch.autograd.grad((y, total), (x, w), (dy, dt))
+    dx, x_bound, dw, w_bound = refs.norm_gradients(x.detach(), w.detach(), dy, dt, 1e-6)
+    # (a gradient below bf16's normal numbers is off by half of its smallest step)
+    assert ((gx.double() - dx).abs() <= x_bound + 2.0 ** -134).all() and ((gw.double() - dw).abs() <= w_bound).all()
+    (q, s), y8, _ = rms_norm_fp8(x.detach(), w.detach())
+    scale = s.double().repeat_interleave(128, 1)
+    assert torch.equal(y8, y) and ((q.double() * scale - exact).abs() <= (refs.E4M3 + refs.NORM) * exact.abs() + 2.0 ** -10 * scale).all()

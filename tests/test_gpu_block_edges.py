@@ -233,3 +233,35 @@ def test_few_tokens_are_not_captured_before_the_weights_are_quantised():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+# ---- rows whose squares are no floats ------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("h", [128, 1032, 7168, 12000])
+@pytest.mark.parametrize("wide", [False, True])
+def test_norm_of_large_rows(h, wide):
+    """Rows from 2^10 to the largest bf16 beside ordinary ones: the norm does not depend on a row's size, and neither do the bounds."""
+    g = torch.Generator(device="cuda").manual_seed(h)
+    x, dy, dt = ((torch.randn(170, h, generator=g, device="cuda")).to(torch.bfloat16) for _ in range(3))
+    for i, power in enumerate((10, 20, 30, 38, 39, 40, 41, 42, 50, 57, 58, 59, 60, 61, 62, 63, 64, 65, 80, 100, 120, 124)):
+        x[5 * i] *= 2.0 ** power
+    x[169, 1:], x[169, 0] = 0, 3e38
+    dt[::2] = 0
+    x.requires_grad_()
+    w = (1 + 0.2 * torch.randn(h, generator=g, device="cuda")).to(torch.float32 if wide else torch.bfloat16).requires_grad_()
+    y, total = rms_norm(x, w, torch.zeros_like(x))
+    exact, _ = refs.norm(x.detach(), w.detach(), 1e-6)
+    assert torch.equal(total, x) and ((y.double() - exact).abs() <= (refs.BF16 + refs.NORM) * exact.abs()).all()
+    alone = rms_norm(x, w)
+    assert torch.equal(alone, y)
+    gx, gw = torch.autograd.grad((y, total), (x, w), (dy, dt), retain_graph=True)
+    dx, x_bound, dw, w_bound = refs.norm_gradients(x.detach(), w.detach(), dy, dt, 1e-6)
+    # (a gradient below bf16's normal numbers is off by half of its smallest step)
+    assert ((gx.double() - dx).abs() <= x_bound + 2.0 ** -134).all(), ((gx.double() - dx).abs() / (x_bound + 2.0 ** -134)).max().item()
+    assert ((gw.double() - dw).abs() <= w_bound).all()
+    (gx,) = torch.autograd.grad(alone, x, dy)
+    dx, x_bound, _, _ = refs.norm_gradients(x.detach(), w.detach(), dy, None, 1e-6)
+    assert ((gx.double() - dx).abs() <= x_bound + 2.0 ** -134).all()
+    if h % 128 == 0:
+        (q, s), y8, _ = rms_norm_fp8(x.detach(), w.detach())
+        scale = s.double().repeat_interleave(128, 1)
+        assert torch.equal(y8, y) and ((q.double() * scale - exact).abs() <= (refs.E4M3 + refs.NORM) * exact.abs() + 2.0 ** -10 * scale).all()
