@@ -236,7 +236,7 @@ def test_few_tokens_are_not_captured_before_the_weights_are_quantised():
 
 
 # ---- rows whose squares are no floats ------------------------------------------------------------------------------------------------------
-@pytest.mark.parametrize("h", [128, 1032, 7168, 12000])
+@pytest.mark.parametrize("h", [128, 1032, 7168, 12000, 20000])
 @pytest.mark.parametrize("wide", [False, True])
 def test_norm_of_large_rows(h, wide):
     """Rows from 2^10 to the largest bf16 beside ordinary ones: the norm does not depend on a row's size, and neither do the bounds."""
