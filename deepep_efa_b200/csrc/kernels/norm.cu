@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
     }
-    // A warp with large values sums their squares times 2^-160 and says so by the sign.
+    // A warp with large values sums their squares times 2^-160 and says so by the sign. (2^-160 itself is no float: factors of 2^-80 one after the other.)
     const bool large = __any_sync(0xffffffffu, sum > kLargeSum);
     if (large) {
         sum = 0.f;
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(1024) rms_norm_kernel(const NormArgs a) {
     const float part = lane < threads / 32 ? s_sum[lane] : 0.f;
     sum = warp_add(part < 0.f ? 0.f : part);
     float r = rsqrtf(sum / (float)a.hidden + a.eps);
-    if (__any_sync(0xffffffffu, part < 0.f)) r = kDown * rsqrtf(fmaf(sum, kDown * kDown, warp_add(part < 0.f ? -part : 0.f)) / (float)a.hidden + a.eps * kDown * kDown);
+    if (__any_sync(0xffffffffu, part < 0.f)) r = kDown * rsqrtf((sum * kDown * kDown + warp_add(part < 0.f ? -part : 0.f)) / (float)a.hidden + a.eps * kDown * kDown);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
         const int i = c * threads + tid;

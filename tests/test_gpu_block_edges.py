@@ -265,3 +265,17 @@ def test_norm_of_large_rows(h, wide):
         (q, s), y8, _ = rms_norm_fp8(x.detach(), w.detach())
         scale = s.double().repeat_interleave(128, 1)
         assert torch.equal(y8, y) and ((q.double() * scale - exact).abs() <= (refs.E4M3 + refs.NORM) * exact.abs() + 2.0 ** -10 * scale).all()
+
+
+@pytest.mark.parametrize("rows,h", [(100, 2048), (100, 7168), (600, 264), (600, 2048), (600, 4096)])
+def test_norm_of_rows_that_are_large_in_parts(rows, h):
+    """Rows whose warps lie on both sides of where squares are summed in another scale: all of them count."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, h, generator=g, device="cuda")
+    x *= 2.0 ** torch.linspace(45, 51, rows, device="cuda")[:, None]
+    half = (torch.arange(h, device="cuda") // 256) % 2 == 0  # (a warp's channels, where a thread has eight)
+    x[::2, half] *= 0.5
+    x, w = x.to(torch.bfloat16), torch.ones(h, device="cuda")
+    y = rms_norm(x, w)
+    exact, _ = refs.norm(x, w, 1e-6)
+    assert ((y.double() - exact).abs() <= (refs.BF16 + refs.NORM) * exact.abs()).all()
