@@ -3,9 +3,10 @@
 //   h[p]   = weights[p] silu(G[e] x[t]) * (U[e] x[t])      p = (t, k), e = idx[t, k]: rows of G and U against the tokens of their expert
 //   out[t] = sum_k W2[e] h[t, k]
 //
-// Bound by reading the chosen experts' weights once. 32 rows of weights (16 of gate and the 16 of up that go with them, or 32 of W2) are multiplied with the
-// selections of one expert, up to eight at a time: the rows are the M operand of mma.sync m16n8k16, the selections its eight columns. (tcgen05 multiplies 128 rows at
-// the least and takes both operands in one type: here weights in e4m3 meet activations of 16 bits, and tiles of 128 rows leave most SMs without work where a token
+// Bound by reading the chosen experts' weights, as long as an expert has up to eight selections. 32 rows of weights (16 of gate and the 16 of up that go with them, or 32
+// of W2) are multiplied with the selections of one expert, up to eight at a time: the rows are the M operand of mma.sync m16n8k16, the selections its eight columns. Past
+// eight an expert's boxes are loaded and multiplied again for every eight (32 tokens on 8 experts of 4096 -> 1408, bf16, us: top-2 60, top-8 108, for 42 of reading them
+// once; 7168 -> 2048, FP8: 89, 222, 54). (tcgen05 multiplies 128 rows at the least and takes both operands in one type: here weights in e4m3 meet activations of 16 bits, and tiles of 128 rows leave most SMs without work where a token
 // meets eight experts. The tensor cores are idle most of the time either way.)
 //
 // A warp is a pipeline of its own: it takes its share of the boxes (128 bytes of each of 32 rows, 4 KB, one TMA copy with 128-byte swizzle) through a ring that only it

@@ -16,7 +16,7 @@ Two execution paths share the structure:
   GEMM's epilogue stores every output row straight into the stage of the token's home rank over NVLink, so the
   combine that remains is a cross-rank flag exchange and a local weighted sum.
 * **a few tokens**: ``forward_few_tokens`` is a decode step of up to 32 tokens on a rank that has all experts: no dispatch and no combine, two
-  kernels that read the chosen experts' weights once.
+  kernels that do little but read the chosen experts' weights.
 
 ``MoEBlock`` puts a layer into a residual stream: addition, root-mean-square norm, choice of the experts, experts.
 
@@ -383,7 +383,8 @@ class MoEBlock(nn.Module):
 
     @torch.no_grad()
     def forward_few_tokens(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None, fp8: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
-        """Decode of up to 32 tokens on a rank that holds every expert (see :meth:`MoELayer.forward_few_tokens`); it can be captured into a graph."""
+        """Decode of up to 32 tokens on a rank that holds every expert (see :meth:`MoELayer.forward_few_tokens`); it can be captured into a graph once ``prepare_fp8`` of
+        the layer has run. Ranks that share the experts call :func:`rms_norm`, ``moe.choose`` and ``moe.forward_low_latency``."""
         y, total = (rms_norm(x, self.norm, eps=self.eps), x) if residual is None else rms_norm(x, self.norm, residual, self.eps)
         return self.moe.forward_few_tokens(y, *self.moe.choose(y), fp8=fp8), total
 

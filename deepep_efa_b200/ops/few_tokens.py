@@ -1,6 +1,6 @@
 """A layer of routed SwiGLU experts for a few tokens, without dispatch and combine (kernels in csrc/kernels/few_tokens.cu).
 
-A decode step of up to 32 tokens whose experts are on this GPU is bound by reading the chosen experts' weights once; this form does little else. The reference
+A decode step of up to 32 tokens whose experts are on this GPU is bound by reading the chosen experts' weights; this form does little else. The reference
 is a communication library and has no counterpart; users of its low-latency pair run the experts between dispatch and combine.
 """
 from __future__ import annotations
@@ -20,9 +20,12 @@ def few_token_experts(x: torch.Tensor, topk_idx: torch.Tensor, topk_weights: tor
     """``out[t] = sum_k topk_weights[t, k] * w2[e] @ (silu(gate[e] @ x[t]) * (up[e] @ x[t]))`` with ``e = topk_idx[t, k] - first_expert``; bf16 ``[T, H]``.
 
     ``x`` bf16 ``[T, H]``, ``T`` up to 32; ``topk_idx`` int64 and ``topk_weights`` fp32 ``[T, K]``. ``w13`` ``[L, 2 I, H]`` holds gate above up, ``w2`` is ``[L, H, I]``: bf16
-    (``H``, ``I`` multiples of 8), or e4m3 with fp32 scales per block of 128 x 128 (``MoELayer.prepare_fp8``; multiples of 128). Activations stay in bf16 in both
-    cases: the hidden values, their weights included, are rounded to it once, sums are in fp32. Ids without an expert in ``[first_expert, first_expert + L)`` are
-    skipped, so ranks that share the experts each compute their part of the sum. Forward only; no host synchronisation, so a step can be captured into a graph."""
+    (``H``, ``I`` multiples of 8), or e4m3 with fp32 scales per block of 128 x 128 (``MoELayer.prepare_fp8``; multiples of 128). Sums are in fp32. Hidden values, their
+    weights included, are kept as two bf16 numbers (16 bits) next to bf16 weights, as fp16 with a power of two per 16 values (11 bits; 2^-24 of the largest of 128) next
+    to e4m3 ones, where ``x`` too is fp16 over a power of two per token (exact to 2^-17 of a token's largest magnitude, off by at most 2^-25 of it below). Ids without
+    an expert in ``[first_expert, first_expert + L)`` are skipped, so ranks that share the experts each compute their part of the sum. Forward only; no host
+    synchronisation, so a step can be captured into a graph. A copy that does not come within two seconds ends the call with a wrong result and sets the
+    device's error word, which ``Buffer.check_status(sync=True)`` reads (a capture before any other call of the library on that device has none)."""
     if x.is_cuda:
         return _ext.load().few_tokens(x, topk_idx, topk_weights, w13, w2, w13_scales, w2_scales, first_expert, out)
     if torch.is_grad_enabled() and (x.requires_grad or topk_weights.requires_grad or w13.requires_grad or w2.requires_grad):
